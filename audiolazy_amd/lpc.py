@@ -56,6 +56,8 @@ def kautocor_frames(sig, frame_len, order, hop=None, device=0, fused=False, exac
   hop = frame_len if hop is None else hop
   if type(sig).__module__.startswith("torch"):
     import torch
+    if not sig.is_cuda or sig.dtype != torch.float64:
+      raise ValueError("a torch signal must be a float64 CUDA tensor")
     flat = sig.reshape(-1)
     F = _frame_count(flat.numel(), frame_len, hop)
     if out is not None:

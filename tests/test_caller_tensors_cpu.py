@@ -1,0 +1,61 @@
+"""The torch entry points take a caller's tensors by address, so what the kernels assume about them -- place, item type, extent,
+order -- is checked on the host before any library call.  The library is a stub here that records its calls: a refusal must come
+before the first of them.  ``dev`` makes a host tensor that says it lies on a device."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from audiolazy_amd import _ffi
+from audiolazy_amd.lpc import kautocor_frames
+
+
+class _Dev(torch.Tensor):
+  is_cuda = True
+
+
+_Dev.__module__ = "torch"      # (the entry points tell tensors from arrays by the type's module)
+
+
+def dev(shape, dtype=torch.float64):
+  return torch.zeros(shape, dtype=dtype).as_subclass(_Dev)
+
+
+class _Lib(object):
+  def __init__(self):
+    self.calls = []
+
+  def __getattr__(self, name):
+    def entry(*args):
+      self.calls.append((name, args))
+      return 0
+    return entry
+
+
+@pytest.fixture
+def lib(monkeypatch):
+  stub = _Lib()
+  monkeypatch.setattr(_ffi, "load", lambda: stub)
+  monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+  return stub
+
+
+# ---- lpc.kautocor_frames ------------------------------------------------------------------------
+@pytest.mark.parametrize("sig", [torch.zeros(960, dtype=torch.float64), torch.zeros((2, 480), dtype=torch.float64),
+                                 dev(960, torch.float32), dev(960, torch.int64), dev(960, torch.bfloat16)],
+                         ids=["host", "host-2d", "float32", "int64", "bfloat16"])
+@pytest.mark.parametrize("with_out", [False, True])
+def test_kautocor_frames_refuses_other_signals(lib, sig, with_out):
+  out = (dev((2, 9)), dev(2), dev(2, torch.int32)) if with_out else None
+  with pytest.raises(ValueError):
+    kautocor_frames(sig, 480, 8, out=out)
+  assert not lib.calls
+
+
+def test_kautocor_frames_hands_over_the_signal(lib):
+  sig = dev(960)
+  coefs, err, status = kautocor_frames(sig, 480, 8)
+  (name, args), = lib.calls
+  assert name == "alz_lpc_kautocor_dev_ex" and args[:5] == (sig.data_ptr(), 2, 480, 480, 8)
+  assert args[5:8] == (coefs.data_ptr(), err.data_ptr(), status.data_ptr())
