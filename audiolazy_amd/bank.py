@@ -140,7 +140,8 @@ def call_sections(sections, seq, memory=None, zero=0., block=None, input_map=Non
 
 
 def mix_sets(y, n_sets, n_inputs, layout="time", out=None, device=0):
-  """Ordered sum over the leading ``n_sets`` groups of ``n_inputs`` channels (alz_mix_dev)."""
+  """Ordered sum over the leading ``n_sets`` groups of ``n_inputs`` channels (alz_mix_dev).  ``out``: the result's own
+  array -- for a torch block a contiguous float64 tensor of the result's shape on the block's device."""
   L = _ffi.load()
   lay = LAYOUTS[layout]
   if _is_torch(y):
@@ -151,7 +152,13 @@ def mix_sets(y, n_sets, n_inputs, layout="time", out=None, device=0):
     if ch != n_sets * n_inputs:
       raise ValueError("block has %d channels, expected %d sets x %d inputs" % (ch, n_sets, n_inputs))
     shape = (n, n_inputs) if lay == _ffi.TIME_MAJOR else (n_inputs, n)
-    res = torch.empty(shape, dtype=torch.float64, device=y.device) if out is None else out
+    if out is None:
+      res = torch.empty(shape, dtype=torch.float64, device=y.device)
+    else:       # the kernel writes n * n_inputs doubles through out.data_ptr(): it must be exactly that buffer
+      if (not getattr(out, "is_cuda", False) or out.dtype != torch.float64 or not out.is_contiguous()
+          or tuple(out.shape) != shape or out.device != y.device):
+        raise ValueError("out must be a contiguous %s float64 CUDA tensor on the block's device" % (shape,))
+      res = out
     ldy, ldo = (ch, n_inputs) if lay == _ffi.TIME_MAJOR else (n, n)
     stream = torch.cuda.current_stream(y.device).cuda_stream
     _ffi.check(L.alz_mix_dev(y.data_ptr(), n_sets, n_inputs, n, lay, ldy, ldo, res.data_ptr(),

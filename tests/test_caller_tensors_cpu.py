@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from audiolazy_amd import _ffi
+from audiolazy_amd.bank import mix_sets
 from audiolazy_amd.lpc import kautocor_frames
 
 
@@ -59,3 +60,27 @@ def test_kautocor_frames_hands_over_the_signal(lib):
   (name, args), = lib.calls
   assert name == "alz_lpc_kautocor_dev_ex" and args[:5] == (sig.data_ptr(), 2, 480, 480, 8)
   assert args[5:8] == (coefs.data_ptr(), err.data_ptr(), status.data_ptr())
+
+
+# ---- mix_sets / FilterBank.mixdown --------------------------------------------------------------
+# 3 sets of 4 inputs, 10 samples: the mix is 40 doubles
+@pytest.mark.parametrize("layout", ["time", "chan"])
+@pytest.mark.parametrize("kind", ["short", "long", "flat", "transposed", "float32", "strided", "host", "array"])
+def test_mix_sets_refuses_other_results(lib, layout, kind):
+  shape = (10, 4) if layout == "time" else (4, 10)
+  y = dev((10, 12) if layout == "time" else (12, 10))
+  out = {"short": lambda: dev((shape[0] - 1, shape[1])), "long": lambda: dev((shape[0] + 1, shape[1])), "flat": lambda: dev(40),
+         "transposed": lambda: dev(shape[::-1]), "float32": lambda: dev(shape, torch.float32),
+         "strided": lambda: dev((shape[0], 2 * shape[1]))[:, ::2], "host": lambda: torch.zeros(shape, dtype=torch.float64),
+         "array": lambda: np.zeros(shape)}[kind]()
+  with pytest.raises(ValueError):
+    mix_sets(y, 3, 4, layout=layout, out=out)
+  assert not lib.calls
+
+
+@pytest.mark.parametrize("layout", ["time", "chan"])
+def test_mix_sets_writes_the_callers_result(lib, layout):
+  out = dev((10, 4) if layout == "time" else (4, 10))
+  assert mix_sets(dev((10, 12) if layout == "time" else (12, 10)), 3, 4, layout=layout, out=out) is out
+  (name, args), = lib.calls
+  assert name == "alz_mix_dev" and args[7] == out.data_ptr()
