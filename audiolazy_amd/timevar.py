@@ -163,7 +163,8 @@ def process_block(b, a, x, xh=None, yh=None, zero=0., layout="time"):
 
   b / a : per delay, a float or a float64 torch CUDA tensor of shape [N] (shared by all channels)
           or matching ``x`` (per channel).  x : float64 CUDA tensor [N, C] ("time") or [C, N].
-  xh / yh : [nb-1, C] / [na-1, C] CUDA tensors, updated in place (None: zeros, not returned).
+  xh / yh : contiguous float64 CUDA tensors [nb-1, C] / [na-1, C], updated in place (None: filled with ``zero``, not
+            returned).
   """
   import torch
   L = _ffi.load()
@@ -193,6 +194,11 @@ def process_block(b, a, x, xh=None, yh=None, zero=0., layout="time"):
         arr[k] = _ffi.TvTap(float(v), None, 0, 0, 0)
     return arr
   tb, ta = taps(b), taps(a)
+  for name, hist, rows in (("xh", xh, nb - 1), ("yh", yh, na - 1)):
+    # (the kernels update [taps - 1, C] doubles in place through its address)
+    if hist is not None and (not getattr(hist, "is_cuda", False) or hist.dtype != torch.float64 or not hist.is_contiguous()
+                             or tuple(hist.shape) not in ((rows, C), (max(rows, 1), C)) or hist.device != x.device):
+      raise ValueError("%s must be a contiguous [%d, %d] float64 CUDA tensor on x's device" % (name, rows, C))
   if xh is None:
     xh = torch.full((max(nb - 1, 1), C), float(zero), dtype=torch.float64, device=x.device)
   if yh is None:

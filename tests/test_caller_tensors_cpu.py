@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from audiolazy_amd import _ffi
+from audiolazy_amd import _ffi, timevar
 from audiolazy_amd.bank import mix_sets
 from audiolazy_amd.lpc import kautocor_frames
 
@@ -84,3 +84,28 @@ def test_mix_sets_writes_the_callers_result(lib, layout):
   assert mix_sets(dev((10, 12) if layout == "time" else (12, 10)), 3, 4, layout=layout, out=out) is out
   (name, args), = lib.calls
   assert name == "alz_mix_dev" and args[7] == out.data_ptr()
+
+
+# ---- timevar.process_block ----------------------------------------------------------------------
+# 3 numerator and 2 denominator taps, 10 samples of 4 channels: xh is [2, 4], yh is [1, 4]
+@pytest.mark.parametrize("layout", ["time", "chan"])
+@pytest.mark.parametrize("side", ["xh", "yh"])
+@pytest.mark.parametrize("kind", ["rows", "columns", "flat", "transposed", "float32", "strided", "host", "array"])
+def test_process_block_refuses_other_histories(lib, layout, side, kind):
+  rows = {"xh": 2, "yh": 1}[side]
+  bad = {"rows": lambda: dev((rows - 1, 4)), "columns": lambda: dev((rows, 3)), "flat": lambda: dev(rows * 4),
+         "transposed": lambda: dev((4, rows)), "float32": lambda: dev((rows, 4), torch.float32),
+         "strided": lambda: dev((rows, 8))[:, ::2], "host": lambda: torch.zeros((rows, 4), dtype=torch.float64),
+         "array": lambda: np.zeros((rows, 4))}[kind]()
+  with pytest.raises(ValueError):
+    timevar.process_block([1., .5, .25], [1., .5], dev((10, 4) if layout == "time" else (4, 10)), layout=layout, **{side: bad})
+  assert not lib.calls
+
+
+@pytest.mark.parametrize("nb,na", [(1, 1), (1, 3), (3, 1), (3, 2)])
+@pytest.mark.parametrize("spare", [0, 1])        # (a side without history: no row, or the one row of the default)
+def test_process_block_takes_the_callers_histories(lib, nb, na, spare):
+  xh, yh = dev((max(nb - 1, spare), 4)), dev((max(na - 1, spare), 4))
+  timevar.process_block([1.] * nb, [1.] * na, dev((10, 4)), xh=xh, yh=yh)
+  (name, args), = lib.calls
+  assert name == "alz_tv_process_dev" and args[11:13] == (xh.data_ptr(), yh.data_ptr())

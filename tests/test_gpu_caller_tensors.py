@@ -41,3 +41,29 @@ def test_mix_sets_into_the_callers_result(alz, layout, n_sets, n_inputs, n):
   out, untouched = guarded((n, n_inputs) if layout == "time" else (n_inputs, n))
   assert mix_sets(torch.from_numpy(y).cuda(), n_sets, n_inputs, layout=layout, out=out) is out
   assert same_bits(out.cpu().numpy(), oracle.mix(y, n_sets, n_inputs, layout=layout)) and untouched()
+
+
+@pytest.mark.parametrize("layout", ["time", "chan"])
+@pytest.mark.parametrize("nb,na", [(1, 1), (1, 3), (3, 1), (3, 2), (6, 4)])
+def test_process_block_updates_the_callers_histories(alz, layout, nb, na):
+  import torch
+  from audiolazy_amd import timevar
+  C, N, cut = 70, 300, 113
+  rng = np.random.default_rng(10 * nb + na)
+  x, s = rng.uniform(-1, 1, (N, C)), rng.uniform(.1, .4, N)
+  b, a = [.5] * (nb - 1), [1.] + [.1] * (na - 1)
+  xh, xh_ok = guarded((nb - 1, C))
+  yh, yh_ok = guarded((na - 1, C))
+  xh.fill_(.25)
+  yh.fill_(.25)
+
+  def part(lo, hi):
+    blk = x[lo:hi] if layout == "time" else x[lo:hi].T
+    y = timevar.process_block([torch.from_numpy(s[lo:hi].copy()).cuda()] + b, a, torch.from_numpy(np.ascontiguousarray(blk)).cuda(),
+                              xh=xh, yh=yh, zero=.25, layout=layout).cpu().numpy()
+    assert xh_ok() and yh_ok()
+    return y if layout == "time" else y.T
+  y = np.concatenate([part(0, cut), part(cut, N)])
+  for ch in (0, 1, 33, 69):
+    assert same_bits(y[:, ch], oracle.tv_df1([s] + b, a, x[:, ch], zero=.25)), ch
+  assert same_bits(xh.cpu().numpy(), x[N - nb + 1:][::-1]) and same_bits(yh.cpu().numpy(), y[N - na + 1:][::-1])
