@@ -10,6 +10,7 @@
 #include <tuple>
 
 #include "alz_common.h"
+#include "alz_host.h"
 
 namespace alz {
 
@@ -82,6 +83,8 @@ struct alz_bank {
   // process_host pipeline: copy-in / compute / copy-out streams and their hand-over events
   hipStream_t host_streams[3] = {nullptr, nullptr, nullptr};
   std::vector<hipEvent_t> host_events;
+  void *host_slot[4] = {nullptr, nullptr, nullptr, nullptr};      // page-locked: two on the way in, two on the way out
+  hipEvent_t slot_events[4] = {nullptr, nullptr, nullptr, nullptr};
   // section pipeline of narrow cascades (process_dev): one stream per section, events per (section, chunk)
   hipStream_t sec_streams[4] = {nullptr, nullptr, nullptr, nullptr};
   std::vector<hipEvent_t> sec_events;
@@ -358,6 +361,10 @@ int alz_bank_destroy(alz_bank_t *h) {
   for (hipStream_t st : h->host_streams)
     if (st) (void)hipStreamDestroy(st);
   for (hipEvent_t ev : h->host_events) (void)hipEventDestroy(ev);
+  for (hipEvent_t ev : h->slot_events)
+    if (ev) (void)hipEventDestroy(ev);
+  for (void *slot : h->host_slot)
+    if (slot) (void)hipHostFree(slot);
   for (hipStream_t st : h->sec_streams)
     if (st) (void)hipStreamDestroy(st);
   for (hipEvent_t ev : h->sec_events) (void)hipEventDestroy(ev);
@@ -885,6 +892,140 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
   return ALZ_OK;
 }
 
+// ---- the host pipeline ----
+// What bounds it is the host's own copying: every byte crosses a page-locked buffer.  4096 channels x 2^16 samples, NumPy in and out
+// (tools/host_path_time.py, profiles/host_path_slots.log): 1 thread 1.8 Gsamples/s, 2 3.1, 4 4.4, 6 4.9, 8 5.2 - 5.4, 12 5.5; buffers of
+// 4 MiB 4.0, 8 MiB 4.9, 16 MiB 5.4, 32 MiB 5.6.  (Page-locking the caller's arrays for the call reached 5.7 without that copy.)
+static constexpr size_t kHostSlot = (size_t)16 << 20;      // bytes of one page-locked buffer
+static constexpr int kHostCopiers = 8;                     // threads per copy, the caller's own among them (fewer on a smaller machine)
+
+// the handle's page-locked buffers, streams and events; false: not to be had (the caller's block takes the synchronous path)
+static bool host_slots(alz_bank_t *h) {
+  for (int i = 0; i < 4; ++i) {
+    if (!h->host_slot[i] && hipHostMalloc(&h->host_slot[i], kHostSlot, hipHostMallocDefault) != hipSuccess) {
+      h->host_slot[i] = nullptr;
+      (void)hipGetLastError();
+      return false;
+    }
+    if (!h->slot_events[i] && hipEventCreateWithFlags(&h->slot_events[i], hipEventDisableTiming) != hipSuccess) {
+      h->slot_events[i] = nullptr;
+      (void)hipGetLastError();
+      return false;
+    }
+  }
+  for (int i = 0; i < 3; ++i)
+    if (!h->host_streams[i] && hipStreamCreateWithFlags(&h->host_streams[i], hipStreamNonBlocking) != hipSuccess) {
+      h->host_streams[i] = nullptr;
+      (void)hipGetLastError();
+      return false;
+    }
+  return true;
+}
+
+// one piece over the link (rows without gaps on both sides are one plain copy)
+static hipError_t queue_rows(void *dst, size_t dpitch, const void *src, size_t spitch, const alz::Pieces &pc, hipMemcpyKind kind,
+                             hipStream_t st) {
+  if (pc.p_rows == 1 || (dpitch == pc.p_width && spitch == pc.p_width))
+    return hipMemcpyAsync(dst, src, pc.p_width * pc.p_rows, kind, st);
+  return hipMemcpy2DAsync(dst, dpitch, src, spitch, pc.p_width, pc.p_rows, kind, st);
+}
+
+static int host_pipeline(alz_bank_t *h, const double *x_host, double *y_host, int64_t n, int layout, int64_t ldx, int64_t ldy,
+                         int64_t lsx, int64_t lsy, uint64_t total_bytes) {
+  const bool tm = layout == ALZ_TIME_MAJOR;
+  int64_t n_chunks = (int64_t)(total_bytes >> 26);            // ~64 MiB of traffic per chunk
+  if (n_chunks < 2) n_chunks = 2;
+  if (n_chunks > 16) n_chunks = 16;
+  const int64_t step = ((n + n_chunks - 1) / n_chunks + 1023) / 1024 * 1024;
+  n_chunks = (n + step - 1) / step;
+  while ((int64_t)h->host_events.size() < 2 * n_chunks) {
+    hipEvent_t ev;
+    if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) != hipSuccess) return fail(ALZ_E_HIP, "hipEventCreate failed");
+    h->host_events.push_back(ev);
+  }
+  hipStream_t s_in = h->host_streams[0], s_run = h->host_streams[1], s_out = h->host_streams[2];
+  const int cores = (int)std::thread::hardware_concurrency();        // (0: not known)
+  alz::CopyCrew crew(ALZ_TUNE("ALZ_HOST_COPIERS", cores > 0 && cores < kHostCopiers ? cores : kHostCopiers) - 1);
+  auto chunk_len = [&](int64_t k) { return (k + 1) * step <= n ? step : n - k * step; };
+  auto width_of = [&](int64_t k, int64_t cols) { return (size_t)(tm ? cols : chunk_len(k)) * 8; };
+  auto rows_of = [&](int64_t k, int64_t chans) { return (size_t)(tm ? chunk_len(k) : chans); };
+  int64_t slot_used[2] = {0, 0};                              // copies queued from the input buffers so far
+  int turn_in = 0;
+  // one piece of chunk k's input: into a buffer that the link has finished with, and on its way
+  auto send = [&](int64_t k, const alz::Pieces &pc) -> bool {
+    const int sl = turn_in;
+    turn_in ^= 1;
+    if (slot_used[sl]++ > 0 && hipEventSynchronize(h->slot_events[sl]) != hipSuccess) return false;
+    const int64_t t0 = k * step;
+    const char *src = (const char *)(tm ? x_host + t0 * ldx : x_host + t0) + pc.p_row * (size_t)ldx * 8 + pc.p_col;
+    char *dst = (char *)(tm ? h->stage_x + t0 * lsx : h->stage_x + t0) + pc.p_row * (size_t)lsx * 8 + pc.p_col;
+    crew.copy(h->host_slot[sl], pc.p_width, src, (size_t)ldx * 8, pc.p_width, pc.p_rows);
+    return queue_rows(dst, (size_t)lsx * 8, h->host_slot[sl], pc.p_width, pc, hipMemcpyHostToDevice, s_in) == hipSuccess &&
+           hipEventRecord(h->slot_events[sl], s_in) == hipSuccess;
+  };
+  // the results: a piece is requested (fetch) one piece before it is copied on to the caller's array (deliver)
+  struct Flight { size_t row, col, rows, width; int64_t t0; int slot; };
+  std::vector<Flight> flights;                                // (at most two: one per output buffer)
+  flights.reserve(2);
+  int turn_out = 0;
+  auto deliver = [&]() -> bool {
+    const Flight f = flights.front();                         // (the older one)
+    flights.erase(flights.begin());
+    if (hipEventSynchronize(h->slot_events[f.slot]) != hipSuccess) return false;
+    char *dst = (char *)(tm ? y_host + f.t0 * ldy : y_host + f.t0) + f.row * (size_t)ldy * 8 + f.col;
+    crew.copy(dst, (size_t)ldy * 8, h->host_slot[f.slot], f.width, f.width, f.rows);
+    return true;
+  };
+  auto fetch = [&](int64_t k, const alz::Pieces &pc) -> bool {
+    if (flights.size() == 2 && !deliver()) return false;
+    const int sl = 2 + turn_out;
+    turn_out ^= 1;
+    const int64_t t0 = k * step;
+    const char *src = (const char *)(tm ? h->stage_y + t0 * lsy : h->stage_y + t0) + pc.p_row * (size_t)lsy * 8 + pc.p_col;
+    flights.push_back(Flight{pc.p_row, pc.p_col, pc.p_rows, pc.p_width, t0, sl});
+    return queue_rows(h->host_slot[sl], pc.p_width, src, (size_t)lsy * 8, pc, hipMemcpyDeviceToHost, s_out) == hipSuccess &&
+           hipEventRecord(h->slot_events[sl], s_out) == hipSuccess;
+  };
+
+  int rc = ALZ_OK;
+  // round k: the input of chunk k and the results of chunk k - 1, piece by piece in turn
+  for (int64_t k = 0; k <= n_chunks && rc == ALZ_OK; ++k) {
+    const bool has_in = k < n_chunks, has_out = k > 0;
+    alz::Pieces in(has_in ? width_of(k, h->n_inputs) : 0, has_in ? rows_of(k, h->n_inputs) : 0, kHostSlot);
+    alz::Pieces out(has_out ? width_of(k - 1, h->channels) : 0, has_out ? rows_of(k - 1, h->channels) : 0, kHostSlot);
+    bool more_in = has_in, more_out = has_out;
+    while ((more_in || more_out) && rc == ALZ_OK) {
+      if (more_in) {
+        more_in = in.next();
+        if (more_in) {
+          if (!send(k, in)) rc = fail(ALZ_E_HIP, "host pipeline: copy-in failed");
+        } else if (hipEventRecord(h->host_events[2 * k], s_in) != hipSuccess ||
+                   hipStreamWaitEvent(s_run, h->host_events[2 * k], 0) != hipSuccess) {
+          rc = fail(ALZ_E_HIP, "host pipeline: copy-in failed");
+        } else {
+          const int64_t t0 = k * step;
+          rc = alz_bank_process_dev(h, tm ? h->stage_x + t0 * lsx : h->stage_x + t0, tm ? h->stage_y + t0 * lsy : h->stage_y + t0,
+                                    chunk_len(k), layout, lsx, lsy, s_run);
+          if (rc == ALZ_OK && (hipEventRecord(h->host_events[2 * k + 1], s_run) != hipSuccess ||
+                               hipStreamWaitEvent(s_out, h->host_events[2 * k + 1], 0) != hipSuccess))
+            rc = fail(ALZ_E_HIP, "host pipeline: hand-over to copy-out failed");
+        }
+      }
+      if (more_out && rc == ALZ_OK) {
+        more_out = out.next();
+        if (more_out && !fetch(k - 1, out)) rc = fail(ALZ_E_HIP, "host pipeline: copy-out failed");
+      }
+    }
+  }
+  while (!flights.empty() && rc == ALZ_OK)
+    if (!deliver()) rc = fail(ALZ_E_HIP, "host pipeline: copy-out failed");
+  const hipError_t e1 = hipStreamSynchronize(s_in), e2 = hipStreamSynchronize(s_run), e3 = hipStreamSynchronize(s_out);
+  if (rc == ALZ_OK && (e1 != hipSuccess || e2 != hipSuccess || e3 != hipSuccess))
+    rc = fail(ALZ_E_HIP, "host pipeline: stream synchronisation failed");
+  if (rc == ALZ_OK) rc = take_look_error(h);
+  return rc;
+}
+
 int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, int64_t n, int layout,
                           int64_t ldx, int64_t ldy) {
   if (!h || !x_host || !y_host) return fail(ALZ_E_ARG, "NULL argument");
@@ -907,70 +1048,14 @@ int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, i
   if (rc) return rc;
   rc = grow(&h->stage_y, &h->stage_y_bytes, (uint64_t)out_rows * lsy * 8);
   if (rc) return rc;
-  // Large blocks: pin the caller's arrays for the call and run copy-in, kernels and copy-out as a
-  // three-stage pipeline over chunks of the time axis (pinned, double-buffered staging).
-  // The link then carries both directions at once and at the pinned rate; small blocks (the filter
-  // call protocol's 4096-sample blocks) keep the plain synchronous path, whose latency is lower.
+  // Large blocks: copy-in, kernels and copy-out as a three-stage pipeline over chunks of the time axis, through page-locked buffers
+  // of the handle (two per direction, kHostSlot bytes each) that a few threads fill and empty.  The link then carries both
+  // directions at once; small blocks (the filter call protocol's 4096-sample blocks) keep the plain synchronous path, whose latency
+  // is lower.  The caller's own arrays are never page-locked: that would change memory the library does not own.
   static const int pipe_env = ALZ_TUNE("ALZ_HOST_PIPE", 1);
   const uint64_t total_bytes = ((uint64_t)in_rows * in_cols + (uint64_t)out_rows * out_cols) * 8;
-  if (pipe_env && total_bytes >= ((uint64_t)64 << 20) && n >= 8192) {
-    const uint64_t x_extent = ((uint64_t)(in_rows - 1) * ldx + in_cols) * 8;
-    const uint64_t y_extent = ((uint64_t)(out_rows - 1) * ldy + out_cols) * 8;
-    const hipError_t rx = hipHostRegister((void *)x_host, x_extent, hipHostRegisterDefault);
-    const bool x_ok = rx == hipSuccess || rx == hipErrorHostMemoryAlreadyRegistered;
-    hipError_t ry = hipErrorUnknown;
-    if (x_ok) ry = hipHostRegister((void *)y_host, y_extent, hipHostRegisterDefault);
-    const bool y_ok = ry == hipSuccess || ry == hipErrorHostMemoryAlreadyRegistered;
-    (void)hipGetLastError();
-    if (x_ok && y_ok) {
-      int64_t n_chunks = (int64_t)(total_bytes >> 26);            // ~64 MiB of traffic per chunk
-      if (n_chunks < 2) n_chunks = 2;
-      if (n_chunks > 16) n_chunks = 16;
-      int64_t step = ((n + n_chunks - 1) / n_chunks + 1023) / 1024 * 1024;
-      n_chunks = (n + step - 1) / step;
-      rc = ALZ_OK;
-      for (int i = 0; i < 3 && rc == ALZ_OK; ++i)
-        if (!h->host_streams[i] && hipStreamCreateWithFlags(&h->host_streams[i], hipStreamNonBlocking) != hipSuccess)
-          rc = fail(ALZ_E_HIP, "hipStreamCreate failed");
-      while (rc == ALZ_OK && (int64_t)h->host_events.size() < 2 * n_chunks) {
-        hipEvent_t ev;
-        if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) != hipSuccess) rc = fail(ALZ_E_HIP, "hipEventCreate failed");
-        else h->host_events.push_back(ev);
-      }
-      hipStream_t s_in = h->host_streams[0], s_run = h->host_streams[1], s_out = h->host_streams[2];
-      const bool tm = layout == ALZ_TIME_MAJOR;
-      for (int64_t k = 0; k < n_chunks && rc == ALZ_OK; ++k) {
-        const int64_t t0 = k * step, len = (t0 + step <= n ? step : n - t0);
-        const double *src = tm ? x_host + t0 * ldx : x_host + t0;
-        double *dst = tm ? h->stage_x + t0 * lsx : h->stage_x + t0;
-        if (hipMemcpy2DAsync(dst, (size_t)lsx * 8, src, (size_t)ldx * 8, (size_t)(tm ? in_cols : len) * 8,
-                             (size_t)(tm ? len : in_rows), hipMemcpyHostToDevice, s_in) != hipSuccess ||
-            hipEventRecord(h->host_events[2 * k], s_in) != hipSuccess ||
-            hipStreamWaitEvent(s_run, h->host_events[2 * k], 0) != hipSuccess) {
-          rc = fail(ALZ_E_HIP, "host pipeline: copy-in failed");
-          break;
-        }
-        rc = alz_bank_process_dev(h, tm ? h->stage_x + t0 * lsx : h->stage_x + t0,
-                                  tm ? h->stage_y + t0 * lsy : h->stage_y + t0, len, layout, lsx, lsy, s_run);
-        if (rc) break;
-        double *out = tm ? y_host + t0 * ldy : y_host + t0;
-        const double *res = tm ? h->stage_y + t0 * lsy : h->stage_y + t0;
-        if (hipEventRecord(h->host_events[2 * k + 1], s_run) != hipSuccess ||
-            hipStreamWaitEvent(s_out, h->host_events[2 * k + 1], 0) != hipSuccess ||
-            hipMemcpy2DAsync(out, (size_t)ldy * 8, res, (size_t)lsy * 8, (size_t)(tm ? out_cols : len) * 8,
-                             (size_t)(tm ? len : out_rows), hipMemcpyDeviceToHost, s_out) != hipSuccess)
-          rc = fail(ALZ_E_HIP, "host pipeline: copy-out failed");
-      }
-      const hipError_t e1 = hipStreamSynchronize(s_in), e2 = hipStreamSynchronize(s_run), e3 = hipStreamSynchronize(s_out);
-      if (rx == hipSuccess) (void)hipHostUnregister((void *)x_host);
-      if (ry == hipSuccess) (void)hipHostUnregister((void *)y_host);
-      if (rc == ALZ_OK && (e1 != hipSuccess || e2 != hipSuccess || e3 != hipSuccess))
-        rc = fail(ALZ_E_HIP, "host pipeline: stream synchronisation failed");
-      if (rc == ALZ_OK) rc = take_look_error(h);
-      return rc;
-    }
-    if (rx == hipSuccess) (void)hipHostUnregister((void *)x_host);     // y could not be pinned: plain path
-  }
+  if (pipe_env && total_bytes >= ((uint64_t)64 << 20) && n >= 8192 && host_slots(h))
+    return host_pipeline(h, x_host, y_host, n, layout, ldx, ldy, lsx, lsy, total_bytes);
   ALZ_HIP_CHECK(hipMemcpy2D(h->stage_x, (size_t)lsx * 8, x_host, (size_t)ldx * 8, (size_t)in_cols * 8,
                             (size_t)in_rows, hipMemcpyHostToDevice));
   rc = alz_bank_process_dev(h, h->stage_x, h->stage_y, n, layout, lsx, lsy, nullptr);

@@ -104,7 +104,10 @@ int alz_bank_get_state(alz_bank_t *h, double *xh_host, double *yh_host);
  *   x: n_inputs channels, y: `channels` channels, both in `layout`;
  *   ldx / ldy: leading dimension in elements (TIME_MAJOR: >= channel count,
  *   CHAN_MAJOR: >= n).  y may alias x only in DIAGONAL mode with ldx == ldy.
- * process_host stages through device buffers owned by the handle.
+ * process_host stages through device buffers owned by the handle, blocks of 64 MiB
+ * (input and output together) and more also through page-locked host buffers of
+ * its own (64 MiB, allocated by the first such call); it returns when the results
+ * are in y.
  * Device scratch is allocated on first need by the call that needs it and kept
  * by the handle (chunk states of the time-parallel mode; for a long feedback-
  * free section on a big time-major block, a slab of one 8-byte start stamp per
