@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64) void k_acorr_lane(const double *__restrict__ si
 // pieces from distinct banks.  Products are formed "by later index" -- a new sample x[m] meets
 // x[m-i] for every lag i -- which adds each lag's terms in the same ascending order as the
 // reference (bit-exact) and needs only the previous chunk(s) as history, all statically indexed.
-// Needs frame starts on 16-byte boundaries (even hop) and P <= 33.
+// Needs frame starts on 16-byte boundaries (even hop), an even frame length and P <= 33.
 __device__ __forceinline__ void lpc_dma16(const void *gsrc, unsigned lds_dst) {
   unsigned keep;
   asm volatile(
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(64) void k_acorr_stage(const double *__restrict__ s
     if (fr > n_frames - 1) fr = n_frames - 1;
     const int piece = (lane % 8) ^ (int)((8 * j + lane / 8) & 7);
     int64_t s0 = (int64_t)16 * c + 2 * piece;
-    if (s0 > L - 2) s0 = (L >= 2) ? ((L - 2) & ~1) : 0;   // keep the (aligned) 16-byte read inside the frame
+    if (s0 > L - 2) s0 = L - 2;               // keep the 16-byte read inside the frame (L is even; nothing past it is summed)
     return sig + fr * hop + s0;
   };
   auto queue = [&](int c) {
@@ -533,8 +533,10 @@ static bool stage_ring2(int64_t) {
   return force != 0;
 }
 
+// (an odd frame's last sample shares its 16 bytes with a double that may lie behind the signal: the staged kernel reads pairs inside
+// the frame only, so odd lengths go to k_acorr_lane)
 static bool stage_ok(const double *sig, int64_t n_frames, int frame_len, int64_t hop) {
-  return n_frames >= 16384 && frame_len >= 32 && (hop % 2) == 0 && ((uintptr_t)sig & 15) == 0;
+  return n_frames >= 16384 && frame_len >= 32 && (frame_len % 2) == 0 && (hop % 2) == 0 && ((uintptr_t)sig & 15) == 0;
 }
 
 static acorr_lane_fn pick_acorr_lane(int P) {

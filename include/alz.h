@@ -198,9 +198,10 @@ int alz_lpc_kautocor_dev(const double *sig_dev, int64_t n_frames, int frame_len,
 /* The same with options.  ALZ_LPC_FUSED: the autocorrelation sums use one fused multiply-add per term
  * instead of a separately rounded multiply and add (the kernel is bound by FP64 issue: half the
  * instructions).  Same ascending order per lag; the lags are then NOT bit-identical to
- * lazy_analysis.py:311-312 (relative differences ~1e-16; contract 1e-6).  Needs frames of >= 32
- * samples, an even hop, >= 16384 frames and a curated order (8, 10, 12, 16, 20, 24, 32); other shapes
- * run the exact kernels whatever the flag says.  No reference counterpart (CPython never fuses). */
+ * lazy_analysis.py:311-312 (relative differences ~1e-16; contract 1e-6).  Needs an even frame
+ * length of >= 32 samples, an even hop, >= 16384 frames and a curated order (8, 10, 12, 16, 20, 24, 32);
+ * other shapes run the exact kernels whatever the flag says.  No reference counterpart (CPython never
+ * fuses). */
 #define ALZ_LPC_FUSED 1
 /* ALZ_LPC_DENSE: Levinson-Durbin with the reference's own dense inner products in the reference's
  * order (lazy_lpc.py:121-131: inner(a, b) = sum(acdata[|i-j|] * a_i * b_j ...), O(order^3) per frame)
