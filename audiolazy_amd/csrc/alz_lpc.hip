@@ -672,6 +672,7 @@ int alz_lpc_kautocor_dev_ex(const double *sig_dev, int64_t n_frames, int frame_l
                             int order, double *coefs_dev, double *err_dev, int *status_dev, int flags, int device,
                             void *stream) {
   if (!sig_dev || !coefs_dev || !err_dev || !status_dev) return alz::fail(ALZ_E_ARG, "NULL argument");
+  if (n_frames < 0 || frame_len < 1 || hop < 0 || order < 0) return alz::fail(ALZ_E_ARG, "lpc: bad frame geometry");
   int prev = 0;
   ALZ_HIP_CHECK(hipGetDevice(&prev));
   if (prev != device) ALZ_HIP_CHECK(hipSetDevice(device));
@@ -789,6 +790,7 @@ int alz_levinson_dev(const double *r_dev, int64_t n_frames, int n_lags, int orde
 int alz_acorr_dev(const double *sig_dev, int64_t n_frames, int frame_len, int64_t hop, int max_lag,
                   double *r_dev, int device, void *stream) {
   if (!sig_dev || !r_dev) return alz::fail(ALZ_E_ARG, "NULL argument");
+  if (n_frames < 0 || frame_len < 1 || hop < 0 || max_lag < 0) return alz::fail(ALZ_E_ARG, "acorr: bad frame geometry");
   int prev = 0;
   ALZ_HIP_CHECK(hipGetDevice(&prev));
   if (prev != device) ALZ_HIP_CHECK(hipSetDevice(device));

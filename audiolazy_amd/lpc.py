@@ -25,6 +25,8 @@ _DevBuf = _ffi.DevBuf
 
 
 def _frame_count(n_samples, frame_len, hop):
+  if hop < 0:
+    raise ValueError("negative hop")
   return 0 if n_samples < frame_len else (n_samples - frame_len) // hop + 1
 
 
