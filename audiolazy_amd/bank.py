@@ -430,19 +430,27 @@ class FilterBank(object):
     x : [N, n_inputs] (layout="time") or [n_inputs, N] (layout="chan"), float64;
         a NumPy array (staged through the device) or a torch CUDA tensor
         (processed in place in HBM on the current torch stream).
-    Returns an array / tensor of [N, channels] or [channels, N].
+    Returns an array / tensor of [N, channels] or [channels, N]: ``out`` where one is given (float64 of that shape; an
+    array must be C-contiguous, a tensor needs contiguous rows and the input's device).
     """
     lay = LAYOUTS[layout]
     if _is_torch(x):
       return self._process_torch(x, lay, out)
     x = np.ascontiguousarray(x, dtype=np.float64)
-    if x.ndim == 1:
+    flat = x.ndim == 1
+    if flat:
       x = x.reshape(-1, 1) if lay == _ffi.TIME_MAJOR else x.reshape(1, -1)
     n, cin = (x.shape if lay == _ffi.TIME_MAJOR else x.shape[::-1])
     if cin != self.n_inputs:
       raise ValueError("block has %d input channels, bank expects %d" % (cin, self.n_inputs))
     shape = (n, self.channels) if lay == _ffi.TIME_MAJOR else (self.channels, n)
-    y = np.empty(shape) if out is None else out
+    if out is None:
+      y = np.empty(shape)
+    else:       # the library writes n * channels doubles through its address: it must be exactly that buffer
+      if (not isinstance(out, np.ndarray) or out.dtype != np.float64 or not out.flags.c_contiguous or not out.flags.writeable
+          or (out.shape != shape and not (flat and self.channels == 1 and out.shape == (n,)))):
+        raise ValueError("out must be a writable C-contiguous float64 array of shape %s" % (shape,))
+      y = out
     if n == 0:
       return y
     ldx = self.n_inputs if lay == _ffi.TIME_MAJOR else n

@@ -1,6 +1,7 @@
 """The torch entry points take a caller's tensors by address, so what the kernels assume about them -- place, item type, extent,
 order -- is checked on the host before any library call.  The library is a stub here that records its calls: a refusal must come
 before the first of them.  ``dev`` makes a host tensor that says it lies on a device."""
+import ctypes
 import types
 
 import numpy as np
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 from audiolazy_amd import _ffi, timevar
-from audiolazy_amd.bank import mix_sets
+from audiolazy_amd.bank import FilterBank, mix_sets
 from audiolazy_amd.lpc import kautocor_frames
 
 
@@ -109,3 +110,33 @@ def test_process_block_takes_the_callers_histories(lib, nb, na, spare):
   timevar.process_block([1.] * nb, [1.] * na, dev((10, 4)), xh=xh, yh=yh)
   (name, args), = lib.calls
   assert name == "alz_tv_process_dev" and args[11:13] == (xh.data_ptr(), yh.data_ptr())
+
+
+# ---- FilterBank.process on arrays ---------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["time", "chan"])
+@pytest.mark.parametrize("kind", ["short", "transposed", "flat", "float32", "strided", "fortran", "read-only", "tensor", "list"])
+def test_process_refuses_other_results(lib, layout, kind):
+  bank = FilterBank([([1.], [1., .5])], n_inputs=4)
+  del lib.calls[:]
+  shape = (10, 4) if layout == "time" else (4, 10)
+  out = {"short": lambda: np.zeros((shape[0] - 1, shape[1])), "transposed": lambda: np.zeros(shape[::-1]), "flat": lambda: np.zeros(40),
+         "float32": lambda: np.zeros(shape, np.float32), "strided": lambda: np.zeros((shape[0], 2 * shape[1]))[:, ::2],
+         "fortran": lambda: np.zeros(shape, order="F"), "read-only": lambda: np.broadcast_to(np.zeros(shape[1]), shape),
+         "tensor": lambda: torch.zeros(shape, dtype=torch.float64), "list": lambda: [[0.] * shape[1]] * shape[0]}[kind]()
+  with pytest.raises(ValueError):
+    bank.process(np.zeros(shape), layout=layout, out=out)
+  assert not lib.calls
+
+
+@pytest.mark.parametrize("layout", ["time", "chan"])
+def test_process_writes_the_callers_result(lib, layout):
+  def written(bank, x, out):
+    del lib.calls[:]
+    assert bank.process(x, layout=layout, out=out) is out
+    (name, args), = lib.calls
+    return name == "alz_bank_process_host" and ctypes.cast(args[2], ctypes.c_void_p).value == out.ctypes.data
+  shape = (10, 4) if layout == "time" else (4, 10)
+  assert written(FilterBank([([1.], [1., .5])], n_inputs=4), np.zeros(shape), np.zeros(shape))
+  one = FilterBank([([1.], [1., .5])], n_inputs=1)
+  assert written(one, np.zeros(10), np.zeros((10, 1) if layout == "time" else (1, 10)))
+  assert written(one, np.zeros(10), np.zeros(10))        # (a flat block and its flat result)
