@@ -210,8 +210,8 @@ def mix_tracks(tracks, deltas, zero=0., device=0):
     dev = tracks[0].device
     for i, k in enumerate(order):
       t = tracks[k]
-      if not t.is_cuda or t.dtype != torch.float64 or not t.is_contiguous():
-        raise ValueError("tracks must be contiguous float64 CUDA tensors")
+      if not t.is_cuda or t.dtype != torch.float64 or not t.is_contiguous() or t.device != dev:
+        raise ValueError("tracks must be contiguous float64 CUDA tensors on one device")
       ptrs[i] = t.data_ptr()
     out = torch.empty((n_out,), dtype=torch.float64, device=dev)
     stream = torch.cuda.current_stream(dev).cuda_stream
@@ -478,6 +478,8 @@ class FilterBank(object):
   def _process_torch(self, x, lay, out):
     import torch
     ldx = self._row_pitch(x, "input")
+    if (x.device.index or 0) != self.device:
+      raise ValueError("the block is on %s, the bank on device %d" % (x.device, self.device))
     n, cin = (tuple(x.shape) if lay == _ffi.TIME_MAJOR else tuple(x.shape)[::-1])
     if cin != self.n_inputs:
       raise ValueError("block has %d input channels, bank expects %d" % (cin, self.n_inputs))

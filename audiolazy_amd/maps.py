@@ -51,6 +51,8 @@ def map_block(op, x, other=None, p0=0., p1=0., out=None, device=0):
         raise ValueError("torch blocks must be contiguous float64 CUDA tensors")
     if binary and tuple(other.shape) != tuple(x.shape):
       raise ValueError("blocks differ in shape")
+    if binary and other.device != x.device:
+      raise ValueError("blocks are on different devices")
     if out is None:
       res = torch.empty_like(x)
     else:       # the kernel writes x.numel() doubles through out.data_ptr(): it must be exactly that buffer

@@ -160,6 +160,8 @@ class DirectComm(object):
     import torch
     if not (x.is_cuda and x.dtype == torch.float64 and x.is_contiguous()):
       raise ValueError("contiguous float64 CUDA tensors only")
+    if (x.device.index or 0) != self.device:
+      raise ValueError("the tensor is on %s, the communicator on device %d" % (x.device, self.device))
 
   def gather(self, x, dst=None):
     import ctypes

@@ -179,8 +179,8 @@ def process_block(b, a, x, xh=None, yh=None, zero=0., layout="time"):
     arr = (_ffi.TvTap * len(coefs))()
     for k, v in enumerate(coefs):
       if type(v).__module__.startswith("torch"):
-        if not v.is_cuda or v.dtype != torch.float64 or not v.is_contiguous():
-          raise ValueError("coefficient series must be contiguous float64 CUDA tensors")
+        if not v.is_cuda or v.dtype != torch.float64 or not v.is_contiguous() or v.device != x.device:
+          raise ValueError("coefficient series must be contiguous float64 CUDA tensors on x's device")
         keep.append(v)
         if v.dim() == 1:
           if v.numel() != n:

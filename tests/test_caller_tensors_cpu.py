@@ -140,3 +140,47 @@ def test_process_writes_the_callers_result(lib, layout):
   one = FilterBank([([1.], [1., .5])], n_inputs=1)
   assert written(one, np.zeros(10), np.zeros((10, 1) if layout == "time" else (1, 10)))
   assert written(one, np.zeros(10), np.zeros(10))        # (a flat block and its flat result)
+
+
+# ---- one device for the tensors of a call -------------------------------------------------------
+class _Elsewhere(_Dev):
+  device = torch.device("cuda", 1)
+
+
+_Elsewhere.__module__ = "torch"
+
+
+def elsewhere(*args, **kw):
+  return dev(*args, **kw).as_subclass(_Elsewhere)
+
+
+def test_tensors_of_another_device_are_refused(lib):
+  from audiolazy_amd import sharding
+  from audiolazy_amd.bank import mix_tracks
+  from audiolazy_amd.maps import map_block
+  bank = FilterBank([([1.], [1., .5])], n_inputs=4)            # (a bank of device 0)
+  comm = sharding.DirectComm(0, 1, bytes(128), device=0)
+  del lib.calls[:]
+  for call in (lambda: bank.process(elsewhere((10, 4))), lambda: bank.process(dev((10, 4)), out=elsewhere((10, 4))),
+               lambda: map_block("add2", dev(10), other=elsewhere(10)), lambda: map_block("abs", dev(10), out=elsewhere(10)),
+               lambda: mix_tracks([dev(10), elsewhere(10)], [0, 3]), lambda: mix_sets(dev((10, 12)), 3, 4, out=elsewhere((10, 4))),
+               lambda: timevar.process_block([elsewhere(10)], [1., .5], dev((10, 4))),
+               lambda: timevar.process_block([1.], [1., elsewhere((10, 4))], dev((10, 4))),
+               lambda: timevar.process_block([1., .5], [1.], dev((10, 4)), xh=elsewhere((1, 4))),
+               lambda: kautocor_frames(dev(960), 480, 8, out=(elsewhere((2, 9)), dev(2), dev(2, torch.int32))),
+               lambda: comm.gather(elsewhere(10)), lambda: comm.sum(elsewhere(10))):
+    with pytest.raises(ValueError):
+      call()
+    assert not lib.calls
+
+
+def test_tensors_of_the_banks_device_are_taken(lib):
+  from audiolazy_amd.bank import mix_tracks
+  from audiolazy_amd.maps import map_block
+  bank = FilterBank([([1.], [1., .5])], n_inputs=4)
+  del lib.calls[:]
+  bank.process(dev((10, 4)), out=dev((10, 4)))
+  map_block("add2", dev(10), other=dev(10), out=dev(10))
+  mix_tracks([dev(10), dev(7), dev(0)], [0, 3, 2])
+  timevar.process_block([dev(10)], [1., dev((10, 4))], dev((10, 4)))
+  assert [name for name, _ in lib.calls] == ["alz_bank_process_dev", "alz_map_dev", "alz_mix_tracks_dev", "alz_tv_process_dev"]
