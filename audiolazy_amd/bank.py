@@ -159,6 +159,8 @@ def mix_sets(y, n_sets, n_inputs, layout="time", out=None, device=0):
           or tuple(out.shape) != shape or out.device != y.device):
         raise ValueError("out must be a contiguous %s float64 CUDA tensor on the block's device" % (shape,))
       res = out
+    if n == 0:
+      return res
     ldy, ldo = (ch, n_inputs) if lay == _ffi.TIME_MAJOR else (n, n)
     stream = torch.cuda.current_stream(y.device).cuda_stream
     _ffi.check(L.alz_mix_dev(y.data_ptr(), n_sets, n_inputs, n, lay, ldy, ldo, res.data_ptr(),
@@ -170,7 +172,7 @@ def mix_sets(y, n_sets, n_inputs, layout="time", out=None, device=0):
     raise ValueError("block has %d channels, expected %d sets x %d inputs" % (ch, n_sets, n_inputs))
   shape = (n, n_inputs) if lay == _ffi.TIME_MAJOR else (n_inputs, n)
   if n == 0:
-    return np.empty(shape)
+    return np.empty(shape) if out is None else out
   ldy, ldo = (ch, n_inputs) if lay == _ffi.TIME_MAJOR else (n, n)
   d_y = _ffi.DevBuf(y.nbytes, device).upload(y)
   d_o = _ffi.DevBuf(n * n_inputs * 8, device)
@@ -214,6 +216,8 @@ def mix_tracks(tracks, deltas, zero=0., device=0):
         raise ValueError("tracks must be contiguous float64 CUDA tensors on one device")
       ptrs[i] = t.data_ptr()
     out = torch.empty((n_out,), dtype=torch.float64, device=dev)
+    if n_out == 0:
+      return out
     stream = torch.cuda.current_stream(dev).cuda_stream
     _ffi.check(L.alz_mix_tracks_dev(nt, ptrs, c_starts, c_lengths, float(zero), n_out, out.data_ptr(),
                                     dev.index or 0, ctypes.c_void_p(stream)))

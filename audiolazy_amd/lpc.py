@@ -73,6 +73,8 @@ def kautocor_frames(sig, frame_len, order, hop=None, device=0, fused=False, exac
       coefs = torch.empty((F, order + 1), dtype=torch.float64, device=sig.device)
       err = torch.empty((F,), dtype=torch.float64, device=sig.device)
       status = torch.empty((F,), dtype=torch.int32, device=sig.device)
+    if F == 0:
+      return coefs, err, status
     stream = torch.cuda.current_stream(sig.device).cuda_stream
     _ffi.check(L.alz_lpc_kautocor_dev_ex(flat.data_ptr(), F, frame_len, hop, order, coefs.data_ptr(),
                                          err.data_ptr(), status.data_ptr(), _lpc_flags(fused, exact),

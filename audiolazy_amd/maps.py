@@ -60,6 +60,8 @@ def map_block(op, x, other=None, p0=0., p1=0., out=None, device=0):
           or tuple(out.shape) != tuple(x.shape) or out.device != x.device):
         raise ValueError("out must be a contiguous float64 CUDA tensor of the input's shape on the input's device")
       res = out
+    if x.numel() == 0:
+      return res
     flags = torch.zeros((1,), dtype=torch.int32, device=x.device)
     stream = torch.cuda.current_stream(x.device).cuda_stream
     _ffi.check(L.alz_map_dev(code, x.data_ptr(), other.data_ptr() if binary else None, float(p0), float(p1),

@@ -60,6 +60,8 @@ def decode_pcm(raw, bits, keep=False, device=0):
       raise ValueError("torch input must be a contiguous uint8 CUDA tensor")
     n = raw.numel() // width
     out = torch.empty((n,), dtype=torch.float64, device=raw.device)
+    if n == 0:
+      return out
     stream = torch.cuda.current_stream(raw.device).cuda_stream
     _ffi.check(L.alz_pcm_decode_dev(raw.data_ptr(), bits, 1 if keep else 0, n, out.data_ptr(),
                                     raw.device.index or 0, ctypes.c_void_p(stream)))
@@ -107,6 +109,8 @@ def encode_pcm(x, dfmt="f", byte_order=None, device=0, _as_array=False):
       raise ValueError("torch input must be a contiguous float64 CUDA tensor")
     n = x.numel()
     out = torch.empty((n * width,), dtype=torch.uint8, device=x.device)
+    if n == 0:
+      return out
     flags = torch.zeros((1,), dtype=torch.int32, device=x.device)
     stream = torch.cuda.current_stream(x.device).cuda_stream
     _ffi.check(L.alz_pcm_encode_dev(x.data_ptr(), n, ord(dfmt), big, out.data_ptr(), flags.data_ptr(),

@@ -204,6 +204,8 @@ def process_block(b, a, x, xh=None, yh=None, zero=0., layout="time"):
   if yh is None:
     yh = torch.full((max(na - 1, 1), C), float(zero), dtype=torch.float64, device=x.device)
   y = torch.empty_like(x)
+  if x.numel() == 0:
+    return y
   ld = C if lay == _ffi.TIME_MAJOR else n
   stream = torch.cuda.current_stream(x.device).cuda_stream
   _ffi.check(L.alz_tv_process_dev(nb, ctypes.cast(tb, ctypes.c_void_p), na, ctypes.cast(ta, ctypes.c_void_p), C,

@@ -184,3 +184,30 @@ def test_tensors_of_the_banks_device_are_taken(lib):
   mix_tracks([dev(10), dev(7), dev(0)], [0, 3, 2])
   timevar.process_block([dev(10)], [1., dev((10, 4))], dev((10, 4)))
   assert [name for name, _ in lib.calls] == ["alz_bank_process_dev", "alz_map_dev", "alz_mix_tracks_dev", "alz_tv_process_dev"]
+
+
+# ---- nothing to do ------------------------------------------------------------------------------
+def test_empty_blocks(lib):
+  """A stream that ends on a block boundary hands over an empty last block: an empty result, like the array forms give."""
+  from audiolazy_amd.bank import mix_tracks
+  from audiolazy_amd.maps import map_block
+  from audiolazy_amd.pcm import decode_pcm, encode_pcm
+  assert tuple(map_block("abs", dev((0, 4))).shape) == (0, 4)
+  assert tuple(map_block("sqrt", dev(0)).shape) == (0,)
+  assert tuple(map_block("add2", dev((4, 0)), other=dev((4, 0))).shape) == (4, 0)
+  out = dev((0, 4))
+  assert map_block("neg", dev((0, 4)), out=out) is out
+  assert tuple(mix_sets(dev((0, 12)), 3, 4).shape) == (0, 4) and tuple(mix_sets(dev((12, 0)), 3, 4, layout="chan").shape) == (4, 0)
+  assert mix_sets(dev((0, 12)), 3, 4, out=out) is out
+  out = np.zeros((0, 4))
+  assert mix_sets(np.zeros((0, 12)), 3, 4, out=out) is out
+  assert tuple(mix_tracks([dev(0)], [0]).shape) == (0,) and tuple(mix_tracks([dev(0), dev(0)], [0, 0]).shape) == (0,)
+  assert tuple(timevar.process_block([1., dev(0)], [1., .5], dev((0, 4))).shape) == (0, 4)
+  assert tuple(timevar.process_block([1.], [1., dev(0)], dev((4, 0)), layout="chan").shape) == (4, 0)
+  raw = decode_pcm(dev(0, torch.uint8), 16)
+  assert tuple(raw.shape) == (0,) and raw.dtype == torch.float64
+  packed = encode_pcm(dev(0), "h")
+  assert tuple(packed.shape) == (0,) and packed.dtype == torch.uint8
+  coefs, err, status = kautocor_frames(dev(479), 480, 8)
+  assert (tuple(coefs.shape), tuple(err.shape), tuple(status.shape)) == ((0, 9), (0,), (0,))
+  assert not lib.calls

@@ -67,3 +67,24 @@ def test_process_block_updates_the_callers_histories(alz, layout, nb, na):
   for ch in (0, 1, 33, 69):
     assert same_bits(y[:, ch], oracle.tv_df1([s] + b, a, x[:, ch], zero=.25)), ch
   assert same_bits(xh.cpu().numpy(), x[N - nb + 1:][::-1]) and same_bits(yh.cpu().numpy(), y[N - na + 1:][::-1])
+
+
+def test_empty_blocks(alz):
+  """An empty block through every torch entry point: an empty result, and the state of the stream as it was."""
+  import torch
+  from audiolazy_amd import maps, pcm, timevar
+  from audiolazy_amd.bank import mix_sets, mix_tracks
+  from audiolazy_amd.lpc import kautocor_frames
+  f64 = lambda *shape: torch.empty(shape, dtype=torch.float64, device="cuda")
+  bank = alz.FilterBank([([1.], [1., .5])], n_inputs=4)
+  bank.reset(zero=.25)
+  assert tuple(bank.process(f64(0, 4)).shape) == (0, 4) and (bank.get_state()[1] == .25).all()
+  assert tuple(maps.map_block("abs", f64(0, 4)).shape) == (0, 4)
+  assert tuple(mix_sets(f64(0, 12), 3, 4).shape) == (0, 4)
+  assert tuple(mix_tracks([f64(0), f64(0)], [0, 0]).shape) == (0,)
+  assert mix_tracks([f64(0), f64(0)], [0, 3], zero=.5).tolist() == [.5] * 3
+  yh = torch.full((1, 4), .25, dtype=torch.float64, device="cuda")
+  assert tuple(timevar.process_block([1., f64(0)], [1., .5], f64(0, 4), yh=yh).shape) == (0, 4) and bool((yh == .25).all())
+  assert tuple(pcm.encode_pcm(f64(0), "h").shape) == (0,)
+  assert tuple(pcm.decode_pcm(torch.empty(0, dtype=torch.uint8, device="cuda"), 24).shape) == (0,)
+  assert tuple(kautocor_frames(f64(479), 480, 8)[0].shape) == (0, 9)
