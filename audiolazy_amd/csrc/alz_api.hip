@@ -1033,6 +1033,9 @@ int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, i
   if (layout != ALZ_TIME_MAJOR && layout != ALZ_CHAN_MAJOR) return fail(ALZ_E_ARG, "bad layout");
   DeviceGuard g(h->device);
   if (!g.ok) return fail(ALZ_E_HIP, "hipSetDevice failed");
+  // A device block of this bank may still be on its way on a stream of the caller's, and its state with it (alz_bank_reset and
+  // alz_bank_set_state wait for the same reason): the streams used below are not ordered behind that one.
+  ALZ_HIP_CHECK(hipDeviceSynchronize());
   // Stage through device buffers with an EVEN leading dimension and 16-byte aligned rows, so
   // the streaming kernels (16-byte DMA pieces) apply whatever pitch the host arrays have.
   const int64_t in_cols = layout == ALZ_TIME_MAJOR ? h->n_inputs : n;
