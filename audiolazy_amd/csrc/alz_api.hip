@@ -83,6 +83,8 @@ struct alz_bank {
   // process_host pipeline: copy-in / compute / copy-out streams and their hand-over events
   hipStream_t host_streams[3] = {nullptr, nullptr, nullptr};
   std::vector<hipEvent_t> host_events;
+  double *pack = nullptr;               // host memory: rows of the synchronous path as the device has them
+  uint64_t pack_bytes = 0;
   void *host_slot[4] = {nullptr, nullptr, nullptr, nullptr};      // page-locked: two on the way in, two on the way out
   hipEvent_t slot_events[4] = {nullptr, nullptr, nullptr, nullptr};
   // section pipeline of narrow cascades (process_dev): one stream per section, events per (section, chunk)
@@ -361,6 +363,7 @@ int alz_bank_destroy(alz_bank_t *h) {
   for (hipStream_t st : h->host_streams)
     if (st) (void)hipStreamDestroy(st);
   for (hipEvent_t ev : h->host_events) (void)hipEventDestroy(ev);
+  free(h->pack);
   for (hipEvent_t ev : h->slot_events)
     if (ev) (void)hipEventDestroy(ev);
   for (void *slot : h->host_slot)
@@ -892,6 +895,52 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
   return ALZ_OK;
 }
 
+// ---- the synchronous host path: a block over the link in one plain copy ----
+// (a two-dimensional copy of pageable rows goes row by row, 8 us each whatever its width: a one-channel block of 4096 samples took
+// 65 ms.  Rows that do not follow each other as the device wants them are laid out in a buffer of the handle first.)
+static double *host_pack(alz_bank_t *h, uint64_t bytes) {
+  if (h->pack_bytes < bytes) {
+    free(h->pack);
+    h->pack = (double *)malloc(bytes);
+    h->pack_bytes = h->pack ? bytes : 0;
+  }
+  return h->pack;
+}
+
+static int rows_to_device(alz_bank_t *h, double *dst, int64_t ldd, const double *src, int64_t lds, int64_t cols, int64_t rows) {
+  const uint64_t bytes = ((uint64_t)(rows - 1) * ldd + cols) * 8;
+  if (lds != ldd && rows > 1) {
+    double *pack = host_pack(h, bytes);
+    if (!pack) {      // (no memory for the layout: row by row)
+      ALZ_HIP_CHECK(hipMemcpy2D(dst, (size_t)ldd * 8, src, (size_t)lds * 8, (size_t)cols * 8, (size_t)rows, hipMemcpyHostToDevice));
+      return ALZ_OK;
+    }
+    for (int64_t r = 0; r < rows; ++r) {
+      memcpy(pack + r * ldd, src + r * lds, (size_t)cols * 8);
+      if (r + 1 < rows && ldd > cols) memset(pack + r * ldd + cols, 0, (size_t)(ldd - cols) * 8);
+    }
+    src = pack;
+  }
+  ALZ_HIP_CHECK(hipMemcpy(dst, src, bytes, hipMemcpyHostToDevice));
+  return ALZ_OK;
+}
+
+static int rows_to_host(alz_bank_t *h, double *dst, int64_t ldd, const double *src, int64_t lds, int64_t cols, int64_t rows) {
+  const uint64_t bytes = ((uint64_t)(rows - 1) * lds + cols) * 8;
+  if (rows > 1 && (ldd != cols || lds != cols)) {      // (what lies between the caller's rows is not ours to write)
+    double *pack = host_pack(h, bytes);
+    if (!pack) {
+      ALZ_HIP_CHECK(hipMemcpy2D(dst, (size_t)ldd * 8, src, (size_t)lds * 8, (size_t)cols * 8, (size_t)rows, hipMemcpyDeviceToHost));
+      return ALZ_OK;
+    }
+    ALZ_HIP_CHECK(hipMemcpy(pack, src, bytes, hipMemcpyDeviceToHost));
+    for (int64_t r = 0; r < rows; ++r) memcpy(dst + r * ldd, pack + r * lds, (size_t)cols * 8);
+    return ALZ_OK;
+  }
+  ALZ_HIP_CHECK(hipMemcpy(dst, src, bytes, hipMemcpyDeviceToHost));
+  return ALZ_OK;
+}
+
 // ---- the host pipeline ----
 // What bounds it is the host's own copying: every byte crosses a page-locked buffer.  4096 channels x 2^16 samples, NumPy in and out
 // (tools/host_path_time.py, profiles/host_path_slots.log): 1 thread 1.8 Gsamples/s, 2 3.1, 4 4.4, 6 4.9, 8 5.2 - 5.4, 12 5.5; buffers of
@@ -1059,15 +1108,13 @@ int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, i
   const uint64_t total_bytes = ((uint64_t)in_rows * in_cols + (uint64_t)out_rows * out_cols) * 8;
   if (pipe_env && total_bytes >= ((uint64_t)64 << 20) && n >= 8192 && host_slots(h))
     return host_pipeline(h, x_host, y_host, n, layout, ldx, ldy, lsx, lsy, total_bytes);
-  ALZ_HIP_CHECK(hipMemcpy2D(h->stage_x, (size_t)lsx * 8, x_host, (size_t)ldx * 8, (size_t)in_cols * 8,
-                            (size_t)in_rows, hipMemcpyHostToDevice));
+  rc = rows_to_device(h, h->stage_x, lsx, x_host, ldx, in_cols, in_rows);
+  if (rc) return rc;
   rc = alz_bank_process_dev(h, h->stage_x, h->stage_y, n, layout, lsx, lsy, nullptr);
   if (rc) return rc;
   ALZ_HIP_CHECK(hipStreamSynchronize(nullptr));
   if (const int lrc = take_look_error(h)) return lrc;
-  ALZ_HIP_CHECK(hipMemcpy2D(y_host, (size_t)ldy * 8, h->stage_y, (size_t)lsy * 8, (size_t)out_cols * 8,
-                            (size_t)out_rows, hipMemcpyDeviceToHost));
-  return ALZ_OK;
+  return rows_to_host(h, y_host, ldy, h->stage_y, lsy, out_cols, out_rows);
 }
 
 int alz_bank_set_fused(alz_bank_t *h, int on) {
