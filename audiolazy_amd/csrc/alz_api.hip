@@ -40,6 +40,34 @@ int ensure_dynamic_lds(const void *fn, int bytes) {
   return ALZ_OK;
 }
 
+bool stream_capturing(hipStream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return status != hipStreamCaptureStatusNone;
+}
+
+int grow_buffer(Kept *kept, bool capturing, double **ptr, uint64_t *have, uint64_t need) {
+  if (*have >= need) return ALZ_OK;
+  if (capturing)
+    return fail(ALZ_E_UNSUPPORTED, "this call needs device scratch, which a stream capture cannot allocate: process one block of this "
+                                   "shape with the bank before the capture");
+  if (*ptr) {
+    if (kept->captured) kept->outgrown.push_back(*ptr);
+    else (void)hipFree(*ptr);
+  }
+  *ptr = nullptr;
+  *have = 0;
+  if (hipMalloc((void **)ptr, need) != hipSuccess) {
+    *ptr = nullptr;
+    return fail(ALZ_E_NOMEM, "hipMalloc failed for " + std::to_string(need) + " bytes");
+  }
+  *have = need;
+  return ALZ_OK;
+}
+
 }  // namespace alz
 
 using alz::fail;
@@ -69,6 +97,7 @@ struct alz_bank {
   // block, and after a set_state whose rows say so (checked there) -- the dot-product zero-state pass of the fused
   // time-parallel cascade chains chunk 0 like every other chunk and needs it (alz_scan.hip)
   bool state_consistent = true;
+  alz::Kept kept;
   std::vector<alz::ScanScratch> scan;   // per section: chunk states and the cached transition matrices
   // a first section with a long numerator as TWO sections that compute the same doubles: its numerator alone (feedback-
   // free) and 1 / its denominator (b = [1]), on the section's own state slabs -- for the time-parallel mode (process_dev)
@@ -113,17 +142,6 @@ struct DeviceGuard {
     if (prev >= 0) (void)hipSetDevice(prev);
   }
 };
-
-int grow(double **ptr, uint64_t *have, uint64_t need) {
-  if (*have >= need) return ALZ_OK;
-  if (*ptr) (void)hipFree(*ptr);
-  *ptr = nullptr;
-  *have = 0;
-  if (hipMalloc((void **)ptr, need) != hipSuccess)
-    return fail(ALZ_E_NOMEM, "hipMalloc failed for " + std::to_string(need) + " bytes");
-  *have = need;
-  return ALZ_OK;
-}
 
 // host [rows = channels][cols] (row-major)  <->  device [cols][channels]
 void transpose_to_dev_order(const double *src, std::vector<double> &dst, int64_t rows, int64_t cols) {
@@ -355,6 +373,7 @@ int alz_bank_destroy(alz_bank_t *h) {
   if (h->stage_x) (void)hipFree(h->stage_x);
   if (h->stage_y) (void)hipFree(h->stage_y);
   if (h->scratch) (void)hipFree(h->scratch);
+  for (void *old : h->kept.outgrown) (void)hipFree(old);
   if (h->map_in) (void)hipFree(h->map_in);
   if (h->expand_in) (void)hipFree(h->expand_in);
   if (h->state_snap) (void)hipFree(h->state_snap);
@@ -503,7 +522,7 @@ int alz_bank_get_state(alz_bank_t *h, double *xh_host, double *yh_host) {
 }
 
 static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, int64_t n, int layout,
-                            int64_t ldx, int64_t ldy, void *stream);
+                            int64_t ldx, int64_t ldy, void *stream, bool capturing);
 
 int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev, int64_t n, int layout,
                          int64_t ldx, int64_t ldy, void *stream) {
@@ -513,21 +532,24 @@ int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev, int6
   // a copy of the bank's state, waits for its own work on `stream`, and on a give-up restores the state and processes the
   // block again with the three-launch form of the same mode (same numerics), so the caller never sees it; an in-place
   // block cannot be processed again (its input is gone): the call FAILS, with the state as it was before the call.
+  // (The one-pass kernel refuses a stream capture: nothing to check there, nothing to wait for.)
+  const bool capturing = h && alz::stream_capturing((hipStream_t)stream);
+  if (capturing) h->kept.captured = true;
   bool snap = false;
   int64_t nx = 0, ny = 0;
-  if (h && h->look_check == ALZ_LOOK_CHECK_CALL && (h->time_parallel == ALZ_TP_AUTO || h->time_parallel == ALZ_TP_ONE_PASS) &&
+  if (h && !capturing && h->look_check == ALZ_LOOK_CHECK_CALL && (h->time_parallel == ALZ_TP_AUTO || h->time_parallel == ALZ_TP_ONE_PASS) &&
       x_dev && y_dev && n >= 4 * alz::kLookChunk && h->channels % 16 == 0) {
     DeviceGuard g(h->device);
     nx = (h->thx > 0 ? h->thx : 1) * h->channels * 2;
     ny = (h->thy > 0 ? h->thy : 1) * h->channels * 2;
-    if (g.ok && grow(&h->state_snap, &h->state_snap_bytes, (uint64_t)(nx + ny) * 8) == ALZ_OK) {
+    if (g.ok && alz::grow_buffer(&h->kept, false, &h->state_snap, &h->state_snap_bytes, (uint64_t)(nx + ny) * 8) == ALZ_OK) {
       hipLaunchKernelGGL(k_state_copy, dim3((unsigned)((nx + ny + 255) / 256)), dim3(256), 0, (hipStream_t)stream, h->state_snap,
                          h->xh_dev, nx, h->state_snap + nx, h->yh_dev, ny);
       snap = hipGetLastError() == hipSuccess;
     }
   }
   if (h) h->look_launched = false;
-  int rc = process_dev_impl(h, x_dev, y_dev, n, layout, ldx, ldy, stream);
+  int rc = process_dev_impl(h, x_dev, y_dev, n, layout, ldx, ldy, stream, capturing);
   if (rc == ALZ_OK && h->look_launched && h->look_check == ALZ_LOOK_CHECK_CALL) {
     DeviceGuard g(h->device);
     ALZ_HIP_CHECK(hipStreamSynchronize((hipStream_t)stream));
@@ -544,7 +566,7 @@ int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev, int6
                                "what it was before this call -- process the block again from a copy of its input");
       const std::string first = h->last_kernels;
       h->no_one_pass = true;
-      rc = process_dev_impl(h, x_dev, y_dev, n, layout, ldx, ldy, stream);
+      rc = process_dev_impl(h, x_dev, y_dev, n, layout, ldx, ldy, stream, false);
       h->no_one_pass = false;
       h->look_reruns += 1;
       h->last_kernels = first + "  [gave up: " + look_site_names(sites) + "; block processed again:] " + h->last_kernels;
@@ -556,7 +578,7 @@ int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev, int6
 }
 
 static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, int64_t n, int layout,
-                            int64_t ldx, int64_t ldy, void *stream) {
+                            int64_t ldx, int64_t ldy, void *stream, bool capturing) {
   if (!h || !x_dev || !y_dev) return fail(ALZ_E_ARG, "NULL argument");
   if (n < 0) return fail(ALZ_E_ARG, "negative block length");
   if (layout != ALZ_TIME_MAJOR && layout != ALZ_CHAN_MAJOR) return fail(ALZ_E_ARG, "bad layout");
@@ -589,6 +611,7 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
       // time-parallel mode: only the one-pass kernel reads through the map (alz_look.hip); where the three-launch form
       // will run, the mapped block comes from a streaming pass as before
       alz::BlockIO probe;
+      probe.kept = &h->kept; probe.capturing = capturing;
       probe.n = n; probe.pre_op = ALZ_MAP_ABS; probe.channels = h->channels; probe.n_inputs = h->n_inputs; probe.n_sets = h->n_sets;
       probe.mode = h->mode; probe.zero = h->zero; probe.fused = h->fused; probe.stream_once = 0;
       probe.look_sync = h->look_check == ALZ_LOOK_CHECK_CALL ? 1 : 0;
@@ -604,7 +627,7 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
     } else {
       const uint64_t extent = layout == ALZ_TIME_MAJOR ? (uint64_t)((n - 1) * ldx + h->n_inputs)
                                                        : (uint64_t)((h->n_inputs - 1) * ldx + n);
-      int rc = grow(&h->map_in, &h->map_in_bytes, extent * 8);
+      int rc = alz::grow_buffer(&h->kept, capturing, &h->map_in, &h->map_in_bytes, extent * 8);
       if (rc) return rc;
       rc = alz::launch_map(h->input_map, x_dev, nullptr, 0.0, 0.0, (int64_t)extent, h->map_in, nullptr, st);
       if (rc) return rc;
@@ -614,6 +637,8 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
   }
 
   alz::BlockIO io;
+  io.kept = &h->kept;
+  io.capturing = capturing;
   io.n = n;
   io.pre_op = 0;
   io.channels = h->channels;
@@ -652,7 +677,7 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
     bool taken = false;
     const char *name = "";
     const int rc = alz::launch_scan_cascade(h->sec.data(), h->n_sections, io, st, h->time_parallel < 0 ? 0 : h->time_parallel,
-                                            &h->scan[(size_t)h->n_sections], h->state_consistent, &taken, &name);
+                                            &h->scan[(size_t)h->n_sections], h->state_consistent && !capturing, &taken, &name);
     if (rc) return rc;
     if (taken) {
       h->state_consistent = true;
@@ -671,7 +696,7 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
     const uint64_t extent = layout == ALZ_TIME_MAJOR ? (uint64_t)n * lde : (uint64_t)h->channels * lde;
     // (a block as large as the output; when the device cannot spare it the bank simply keeps reading by
     // input index through the lane-per-channel kernels: slower, same doubles)
-    if (grow(&h->expand_in, &h->expand_in_bytes, extent * 8) == ALZ_OK) {
+    if (alz::grow_buffer(&h->kept, capturing, &h->expand_in, &h->expand_in_bytes, extent * 8) == ALZ_OK) {
       const int64_t sen = layout == ALZ_TIME_MAJOR ? lde : 1, sec = layout == ALZ_TIME_MAJOR ? 1 : lde;
       const int rc = alz::launch_expand(x_dev, h->expand_in, n, h->channels, h->n_inputs, sxn, sxc, sen, sec, st);
       if (rc) return rc;
@@ -717,7 +742,7 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
       io.c_count = c_count;
       if (generic && io.x == io.y && !alz::comb_takes_in_place(sec, io)) {
         // k_fir / k_generic read their history from the block, so they cannot overwrite it
-        int rc = grow(&h->scratch, &h->scratch_bytes, y_extent * 8);
+        int rc = alz::grow_buffer(&h->kept, capturing, &h->scratch, &h->scratch_bytes, y_extent * 8);
         if (rc) return rc;
         ALZ_HIP_CHECK(hipMemcpyAsync(h->scratch, y_dev, y_extent * 8, hipMemcpyDeviceToDevice, st));
         io.x = h->scratch + t_first * syn;
@@ -1096,9 +1121,9 @@ int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, i
   // contiguous vector keeps the copies one-dimensional and the time-parallel FIR kernel eligible)
   const int64_t lsx = in_cols == 1 ? 1 : (in_cols + 1) & ~(int64_t)1;
   const int64_t lsy = out_cols == 1 ? 1 : (out_cols + 1) & ~(int64_t)1;
-  int rc = grow(&h->stage_x, &h->stage_x_bytes, (uint64_t)in_rows * lsx * 8);
+  int rc = alz::grow_buffer(&h->kept, false, &h->stage_x, &h->stage_x_bytes, (uint64_t)in_rows * lsx * 8);
   if (rc) return rc;
-  rc = grow(&h->stage_y, &h->stage_y_bytes, (uint64_t)out_rows * lsy * 8);
+  rc = alz::grow_buffer(&h->kept, false, &h->stage_y, &h->stage_y_bytes, (uint64_t)out_rows * lsy * 8);
   if (rc) return rc;
   // Large blocks: copy-in, kernels and copy-out as a three-stage pipeline over chunks of the time axis, through page-locked buffers
   // of the handle (two per direction, kHostSlot bytes each) that a few threads fill and empty.  The link then carries both

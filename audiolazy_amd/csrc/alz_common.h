@@ -136,6 +136,17 @@ struct SectionDev {
 };
 
 // Block description handed to the launchers.
+// A graph that captured a process call of a bank holds the addresses of the bank's device scratch.  A bank that has been captured
+// once therefore keeps the buffers it outgrows until it goes, and rebuilds the tables it otherwise keeps between calls in every
+// call: a replay and an eager call do not see of each other which of them wrote the tables last.
+struct Kept {
+  bool captured = false;
+  std::vector<void *> outgrown;
+};
+bool stream_capturing(hipStream_t stream);      // alz_api.hip
+// at least `need` bytes at *ptr (*have: the size it has); not while a capture is going on, which cannot allocate
+int grow_buffer(Kept *kept, bool capturing, double **ptr, uint64_t *have, uint64_t need);
+
 struct BlockIO {
   const double *x;
   double *y;
@@ -154,6 +165,8 @@ struct BlockIO {
                       // honoured by launch_wave and the k_small path of launch_section only
   int look_sync = 0;    // the process call will wait for a one-pass time-parallel launch (ALZ_LOOK_CHECK_CALL): short blocks are
                       // then better off in three launches, which nobody has to wait for (scan_takes_one_pass, ALZ_TP_AUTO)
+  Kept *kept = nullptr;  // the bank's (launch_scan, launch_scan_cascade)
+  bool capturing = false;  // the call is being captured into a graph
   int stream_once = 0;  // the block is large, read once and its result not read again by this call (single-section
                       // bank): k_duo then moves it with non-temporal loads and stores
 };
@@ -214,7 +227,7 @@ int launch_wave_chunks(const SectionDev &sec, const BlockIO &io, hipStream_t str
 // zero-state pass, per-channel scan of the chunk states, replay); opt-in, not bit-exact.
 struct ScanScratch {                 // owned by the bank handle, grown on demand
   double *vxh = nullptr, *vyh = nullptr;
-  uint64_t v_bytes = 0;
+  uint64_t vx_bytes = 0, vy_bytes = 0;
   double *power = nullptr;           // [4][channels] transition matrix A^chunk_len per channel
   uint64_t power_bytes = 0;
   int64_t power_len = 0;             // chunk length the cached matrix belongs to (0: none)

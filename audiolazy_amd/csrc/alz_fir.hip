@@ -867,11 +867,10 @@ int launch_fir(const SectionDev &sec, const BlockIO &io, hipStream_t stream, boo
       p.run_group = W; p.run_span = W * Mc; p.run_first = W * Mc - 1; p.run_first_mul = -1; p.run_stride = -W; p.run_count = Mc;
       FirChains *fc = sec.chains;
       const size_t need = (size_t)(Qc * W * Mc + 1) * gx + 8;
-      // (not while `stream` is being captured: the slab would belong to the graph, and the calls behind it use it too; such a launch
-      // runs free unless an earlier call has made the slab)
-      hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-      if (paced && fc != nullptr && need > fc->len && hipStreamIsCapturing(stream, &capture) == hipSuccess &&
-          capture == hipStreamCaptureStatusNone) {
+      // (a launch that is being captured runs free: a slab allocated there would belong to the graph, and one that the graph only
+      // used could be outgrown and released before a replay)
+      paced = paced && !io.capturing;
+      if (paced && fc != nullptr && need > fc->len) {
         // stream-ordered: the old slab is released behind whatever launch still polls it, the new one
         // exists before this call's kernel -- no device-wide synchronisation inside a process call
         if (fc->flags) (void)hipFreeAsync(fc->flags, stream);

@@ -116,14 +116,8 @@ __global__ __launch_bounds__(256) void k_scan_finish(ScanArgs p) {
   for (int k = 0; k < p.na - 1; ++k) p.yh[(int64_t)k * p.C + c] = p.vyh[(int64_t)k * V + last];
 }
 
-static int grow_scratch(double **ptr, uint64_t *have, uint64_t need) {
-  if (*have >= need) return ALZ_OK;
-  if (*ptr) (void)hipFree(*ptr);
-  *ptr = nullptr;
-  *have = 0;
-  if (hipMalloc((void **)ptr, need) != hipSuccess) return fail(ALZ_E_NOMEM, "hipMalloc failed (time-parallel scratch)");
-  *have = need;
-  return ALZ_OK;
+static int grow_scratch(const BlockIO &io, double **ptr, uint64_t *have, uint64_t need) {
+  return grow_buffer(io.kept, io.capturing, ptr, have, need);
 }
 
 // One pass where the shape allows it (a recursive section, whole 512-sample chunks, either layout since round 5):
@@ -187,6 +181,9 @@ int launch_scan(const SectionDev &sec, int section_index, const BlockIO &io, hip
   if (C % 16) return ALZ_OK;
   const bool one_pass = scan_takes_one_pass(sec, io, chunk_len);
   if (chunk_len < 0) chunk_len = 0;
+  if (one_pass && io.capturing)     // (its launches tell their words in the scratch apart by a key that a replay would repeat)
+    return fail(ALZ_E_UNSUPPORTED, "the one-pass form of the time-parallel mode cannot be captured: set a chunk length (> 0) before the "
+                                   "capture, which means the three-launch form");
   if (one_pass) {
     const int64_t groups = C / 16, Kl = io.n / kLookChunk;
     // (a wait that ran out in an earlier launch is reported by alz_api.hip's take_look_error at every entry point)
@@ -196,19 +193,17 @@ int launch_scan(const SectionDev &sec, int section_index, const BlockIO &io, hip
       for (int k = 0; k < kLookErrWords; ++k) scratch->look_err[k] = 0;
     }
     const uint64_t zneed = look_scratch_bytes(groups, Kl);
-    uint64_t have_z = scratch->zbuf_bytes, have_p = scratch->power_bytes;
-    int rc2 = grow_scratch(&scratch->zbuf, &have_z, zneed);
+    const uint64_t had_p = scratch->power_bytes;
+    int rc2 = grow_scratch(io, &scratch->zbuf, &scratch->zbuf_bytes, zneed);
     if (rc2) return rc2;
-    scratch->zbuf_bytes = have_z;
-    rc2 = grow_scratch(&scratch->power, &have_p, (uint64_t)4 * C * sizeof(double));
+    rc2 = grow_scratch(io, &scratch->power, &scratch->power_bytes, (uint64_t)4 * C * sizeof(double));
+    if (had_p != scratch->power_bytes) scratch->power_len = 0;
     if (rc2) return rc2;
-    if (have_p != scratch->power_bytes) scratch->power_len = 0;
-    scratch->power_bytes = have_p;
     ScanArgs pw;
     pw.x = io.x; pw.sxn = io.sxn; pw.sxc = io.sxc; pw.C = C; pw.n_inputs = io.n_inputs; pw.n_sets = io.n_sets;
     pw.mode = io.mode; pw.map_input = io.map_input; pw.nb = sec.nb; pw.na = sec.na; pw.L = kLookChunk; pw.K = Kl;
     pw.a = sec.a; pw.xh = sec.xh; pw.yh = sec.yh; pw.vxh = nullptr; pw.vyh = nullptr; pw.power = scratch->power;
-    const bool fresh = scratch->power_len != kLookChunk || scratch->power_section != section_index;
+    const bool fresh = io.kept->captured || scratch->power_len != kLookChunk || scratch->power_section != section_index;
     if (fresh) hipLaunchKernelGGL(k_scan_power, dim3((unsigned)((C + 63) / 64)), dim3(64), 0, stream, pw);
     int64_t done = 0;
     rc2 = launch_look(sec, io, stream, scratch->power, scratch->zbuf, zneed, scratch->look_err, &done, kernel_name);
@@ -241,12 +236,10 @@ int launch_scan(const SectionDev &sec, int section_index, const BlockIO &io, hip
   const int64_t V = K * C;
 
   const uint64_t vbytes = (uint64_t)2 * V * sizeof(double);
-  uint64_t have_x = scratch->v_bytes, have_y = scratch->v_bytes;
-  int rc = grow_scratch(&scratch->vxh, &have_x, vbytes);
+  int rc = grow_scratch(io, &scratch->vxh, &scratch->vx_bytes, vbytes);
   if (rc) return rc;
-  rc = grow_scratch(&scratch->vyh, &have_y, vbytes);
+  rc = grow_scratch(io, &scratch->vyh, &scratch->vy_bytes, vbytes);
   if (rc) return rc;
-  scratch->v_bytes = have_x < have_y ? have_x : have_y;
   const bool feedback = sec.na > 1;
 
   ScanArgs p;
@@ -255,11 +248,10 @@ int launch_scan(const SectionDev &sec, int section_index, const BlockIO &io, hip
   p.nb = sec.nb; p.na = sec.na; p.L = L; p.K = K; p.a = sec.a;
   p.xh = sec.xh; p.yh = sec.yh; p.vxh = scratch->vxh; p.vyh = scratch->vyh;
   if (feedback) {
-    uint64_t have_p = scratch->power_bytes;
-    rc = grow_scratch(&scratch->power, &have_p, (uint64_t)4 * C * sizeof(double));
+    const uint64_t had_p = scratch->power_bytes;
+    rc = grow_scratch(io, &scratch->power, &scratch->power_bytes, (uint64_t)4 * C * sizeof(double));
+    if (had_p != scratch->power_bytes) scratch->power_len = 0;
     if (rc) return rc;
-    if (have_p != scratch->power_bytes) scratch->power_len = 0;
-    scratch->power_bytes = have_p;
   }
   p.power = scratch->power;
 
@@ -273,7 +265,7 @@ int launch_scan(const SectionDev &sec, int section_index, const BlockIO &io, hip
     rc = launch_wave_chunks(sec, io, stream, ch, &taken, &inner);
     if (rc) return rc;
     if (!taken) return ALZ_OK;            // (prep only touched scratch)
-    if (scratch->power_len != L || scratch->power_section != section_index) {
+    if (io.kept->captured || scratch->power_len != L || scratch->power_section != section_index) {
       hipLaunchKernelGGL(k_scan_power, dim3((unsigned)((C + 63) / 64)), dim3(64), 0, stream, p);
       scratch->power_len = L;
       scratch->power_section = section_index;
@@ -839,15 +831,12 @@ int launch_scan_cascade(const SectionDev *secs, int nsec, const BlockIO &io, hip
   // scratch: [section][x | y][2 or nb-1][V] + M
   uint64_t need = 0;
   for (int s = 0; s < nsec; ++s) need += (uint64_t)((secs[s].nb - 1) + (secs[s].na - 1)) * V * sizeof(double);
-  uint64_t have = scratch->v_bytes;
-  int rc = grow_scratch(&scratch->vxh, &have, need);
+  int rc = grow_scratch(io, &scratch->vxh, &scratch->vx_bytes, need);
   if (rc) return rc;
-  scratch->v_bytes = have;
-  uint64_t have_p = scratch->power_bytes;
-  rc = grow_scratch(&scratch->power, &have_p, (uint64_t)64 * C * sizeof(double));
+  const uint64_t had_p = scratch->power_bytes;
+  rc = grow_scratch(io, &scratch->power, &scratch->power_bytes, (uint64_t)64 * C * sizeof(double));
+  if (had_p != scratch->power_bytes) scratch->power_len = 0;
   if (rc) return rc;
-  if (have_p != scratch->power_bytes) scratch->power_len = 0;
-  scratch->power_bytes = have_p;
 
   CScanArgs p;
   CascChunks ch;
@@ -887,7 +876,7 @@ int launch_scan_cascade(const SectionDev *secs, int nsec, const BlockIO &io, hip
   if (!ok) return ALZ_OK;
   ch.probe = false;
   p.slot_tm = ch.chunk_major ? 1 : 0;
-  const bool fresh_power = scratch->power_len != L || scratch->power_section != -2;
+  const bool fresh_power = io.kept->captured || scratch->power_len != L || scratch->power_section != -2;
 
   // the zero-state pass: dot products with the cascade's impulse responses where the shape offers them (an OUTER bank
   // reading by input index from rows of chunks: channel-major, or the one contiguous column of a one-stream time-major
@@ -902,13 +891,12 @@ int launch_scan_cascade(const SectionDev *secs, int nsec, const BlockIO &io, hip
   if (dot_pass) {
     // (+ one pair of samples: k_cdot3 requests the responses one pair ahead, also behind the last set's last pair)
     const uint64_t hr_need = ((uint64_t)io.n_sets * L + 2) * 4 * sizeof(double), edge_need = (uint64_t)io.n_sets * 16 * sizeof(double);
-    uint64_t have_h = scratch->hr_bytes, have_e = scratch->edge_bytes;
-    rc = grow_scratch(&scratch->hr, &have_h, hr_need);
+    const uint64_t had_h = scratch->hr_bytes, had_e = scratch->edge_bytes;
+    rc = grow_scratch(io, &scratch->hr, &scratch->hr_bytes, hr_need);
+    if (!rc) rc = grow_scratch(io, &scratch->edge, &scratch->edge_bytes, edge_need);
+    if (had_h != scratch->hr_bytes || had_e != scratch->edge_bytes) scratch->tab_len = 0;
     if (rc) return rc;
-    rc = grow_scratch(&scratch->edge, &have_e, edge_need);
-    if (rc) return rc;
-    const bool fresh_tab = have_h != scratch->hr_bytes || have_e != scratch->edge_bytes || scratch->tab_len != L;
-    scratch->hr_bytes = have_h; scratch->edge_bytes = have_e;
+    const bool fresh_tab = io.kept->captured || scratch->tab_len != L;
     if (fresh_tab) {
       hipLaunchKernelGGL(k_cdot_tables, dim3((unsigned)((io.n_sets + 63) / 64)), dim3(64), 0, stream, p, scratch->hr, scratch->edge);
       scratch->tab_len = L;

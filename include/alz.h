@@ -112,7 +112,14 @@ int alz_bank_get_state(alz_bank_t *h, double *xh_host, double *yh_host);
  * by the handle (chunk states of the time-parallel mode; for a long feedback-
  * free section on a big time-major block, a slab of one 8-byte start stamp per
  * 48 rows and 64 channels -- 1/384 of the block -- through which the waves that
- * share input rows pace each other; nothing is READ through it: same doubles). */
+ * share input rows pace each other; nothing is READ through it: same doubles).
+ * process_dev may be captured into a graph: every replay continues the stream like
+ * the call.  A capture cannot allocate, so a call that needs scratch is refused
+ * there (ALZ_E_UNSUPPORTED) until one block of its shape has been processed, and the
+ * one-pass time-parallel form is refused always (a positive chunk length is not).  A
+ * bank that has been captured keeps outgrown scratch until it is destroyed; destroy
+ * it after its graphs.  Calls and replays of one bank are ordered by the caller,
+ * whichever streams they are on; process_host waits for the device itself. */
 int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev,
                          int64_t n, int layout, int64_t ldx, int64_t ldy,
                          void *stream);
