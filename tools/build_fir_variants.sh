@@ -4,7 +4,7 @@
 set -e
 cd $(dirname $0)/../audiolazy_amd/csrc
 V=../../tools/variants
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -fno-fast-math -DALZ_TUNING"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -fno-fast-math -DALZ_TUNING"
 build() {  # name, defines
   mkdir -p $V/obj_$1
   cp $V/obj_tuning/*.o $V/obj_$1/

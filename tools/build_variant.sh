@@ -9,5 +9,5 @@ V=$R/tools/variants
 mkdir -p $V
 name=$1; src=$2; flags=$3
 obj=$V/${src%.hip}_$name.o
-cd $C && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -fno-fast-math $flags -c $src -o $obj 2>/dev/null &&
+cd $C && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -fno-fast-math $flags -c $src -o $obj 2>/dev/null &&
   /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -Wl,--version-script=alz.map $(ls $C/*.o | grep -v "/${src%.hip}.o") $obj -ldl -o $V/libalzhip_$name.so && echo "built $name"
