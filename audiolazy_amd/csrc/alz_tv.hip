@@ -317,24 +317,10 @@ __device__ __forceinline__ double pick(unsigned long long mask, double yes, doub
   return __longlong_as_double((long long)((a & mask) | (b & ~mask)));
 }
 
-// a load the compiler does not track: the wave waits for it by hand (wait_loaded) so that the
-// next batch can stay in flight across the whole recurrence of the current one
-__device__ __forceinline__ double load_untracked(const double *ptr) {
-  double v;
-  asm volatile("global_load_dwordx2 %0, %1, off" : "=v"(v) : "v"(ptr) : "memory");
-  return v;
-}
-
 template <int NB, int NA, unsigned PB = kTvAny, unsigned PA = kTvAny>
 __global__ __launch_bounds__(64) void k_tv_one(TvArgs p) {
   constexpr bool STATIC = PB != kTvAny;     // compile-time presence masks, as in k_tv
   const int lane = threadIdx.x;
-  constexpr int kLoads = NB + NA;          // loads per batch: x, NB numerator and NA-1 denominator series
-  // Untracked (inline-asm) loads only in the small variant.  Above 256 registers hipcc parks
-  // values in AGPRs right after the asm statement and reuses the VGPR; a load still in flight
-  // would then land in a register that already holds something else (seen as a memory
-  // aperture violation with the 17-tap variant).
-  constexpr bool kUntracked = NB <= 3 && NA <= 3;
   double d[NB], m[NA];
 #pragma unroll
   for (int k = 1; k < NB; ++k) d[k] = (k < p.nb) ? p.xh[k - 1] : 0.0;
@@ -365,25 +351,15 @@ __global__ __launch_bounds__(64) void k_tv_one(TvArgs p) {
   auto fetch = [&](int64_t n0, Batch &t) {
     int64_t i = n0 + lane;
     i = i < p.n ? i : p.n - 1;             // past the end: re-read the last sample (never used)
-    if constexpr (kUntracked) {
-      t.x = load_untracked(p.x + i * p.sxn);
+    t.x = p.x[i * p.sxn];
 #pragma unroll
-      for (int k = 0; k < NB; ++k) t.sb[k] = load_untracked(p.b.series[k] + i * p.b.sn[k]);
+    for (int k = 0; k < NB; ++k) t.sb[k] = p.b.series[k][i * p.b.sn[k]];
 #pragma unroll
-      for (int k = 1; k < NA; ++k) t.sa[k] = load_untracked(p.a.series[k] + i * p.a.sn[k]);
-    } else {
-      t.x = p.x[i * p.sxn];
-#pragma unroll
-      for (int k = 0; k < NB; ++k) t.sb[k] = p.b.series[k][i * p.b.sn[k]];
-#pragma unroll
-      for (int k = 1; k < NA; ++k) t.sa[k] = p.a.series[k][i * p.a.sn[k]];
-    }
+    for (int k = 1; k < NA; ++k) t.sa[k] = p.a.series[k][i * p.a.sn[k]];
   };
-  // the batch fetched before the most recent one has landed once at most kLoads loads (the most
-  // recent batch) plus the y store in between are outstanding; tie the registers to the wait
-  auto wait_loaded = [&](Batch &t) {
-    if constexpr (!kUntracked) return;       // hipcc waits for its own loads
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+  // a use of the batch outside the recurrence's loop: the wait for it (not for the batch behind it, which stays in flight
+  // across the whole recurrence) goes here -- in front of a loop that only reads them, hipcc waits for every load there is
+  auto landed = [&](Batch &t) {
     asm volatile("" : "+v"(t.x));
 #pragma unroll
     for (int k = 0; k < NB; ++k) asm volatile("" : "+v"(t.sb[k]));
@@ -429,17 +405,16 @@ __global__ __launch_bounds__(64) void k_tv_one(TvArgs p) {
   fetch(0, A);
   for (int64_t n0 = 0; n0 < p.n; n0 += 128) {
     fetch(n0 + 64, B);
-    wait_loaded(A);
+    landed(A);
     if (divide) recur(A, n0, std::true_type{});
     else recur(A, n0, std::false_type{});
     fetch(n0 + 128, A);
-    wait_loaded(B);
+    landed(B);
     if (n0 + 64 < p.n) {
       if (divide) recur(B, n0 + 64, std::true_type{});
       else recur(B, n0 + 64, std::false_type{});
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (lane == 0) {
 #pragma unroll
     for (int k = 1; k < NB; ++k)
