@@ -438,6 +438,8 @@ int alz_tv_process_dev(int nb, const alz_tv_tap_t *b, int na, const alz_tv_tap_t
     return alz::fail(ALZ_E_UNSUPPORTED, "time-varying filters are limited to 17 taps per side");
   if ((nb > 1 && !xh_dev) || (na > 1 && !yh_dev)) return alz::fail(ALZ_E_ARG, "history arrays required");
   if (layout != ALZ_TIME_MAJOR && layout != ALZ_CHAN_MAJOR) return alz::fail(ALZ_E_ARG, "unknown layout");
+  if (layout == ALZ_TIME_MAJOR ? (ldx < channels || ldy < channels) : (ldx < n || ldy < n))
+    return alz::fail(ALZ_E_ARG, "row pitch smaller than the row");
   if (a[0].series_dev) return alz::fail(ALZ_E_ARG, "a0 must be constant (normalise a series gain on the host)");
   if (a[0].value == 0.0) return alz::fail(ALZ_E_ZERO_GAIN, "Invalid filter gain");
   alz::TvArgs p;
