@@ -588,6 +588,13 @@ static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, i
     return fail(ALZ_E_ARG, "CHAN_MAJOR leading dimension smaller than the block length");
   if (x_dev == y_dev && (h->mode != ALZ_BANK_DIAGONAL || ldx != ldy))
     return fail(ALZ_E_ARG, "in-place processing needs DIAGONAL mode and ldx == ldy");
+  // One sample per channel, rows of one item without gaps: the block is a time-major row, and that is how the kernels get it (as
+  // strides of 1 and 1 it would pass for a time-major block whose rows are one item wide).
+  if (layout == ALZ_CHAN_MAJOR && n == 1 && ldx == 1 && ldy == 1) {
+    layout = ALZ_TIME_MAJOR;
+    ldx = h->n_inputs;
+    ldy = h->channels;
+  }
   h->last_kernels.clear();
   h->last_kernel = "";
   if (const int lrc = take_look_error(h)) return lrc;      // (an EARLIER block of this handle: read without a sync)
