@@ -171,6 +171,17 @@ struct BlockIO {
                       // bank): k_duo then moves it with non-temporal loads and stores
 };
 
+// A launch has fewer than 2^32 work-items per dimension (more are cut off without an error).  Passes with one per sample go in
+// slices: launch(first, count, blocks) for `items` items of `per_block` each.
+constexpr int64_t kSliceItems = INT64_C(1) << 31;
+template <class F>
+inline void in_slices(int64_t items, int64_t per_block, F launch) {
+  for (int64_t first = 0; first < items; first += kSliceItems) {
+    const int64_t count = items - first < kSliceItems ? items - first : kSliceItems;
+    launch(first, count, (unsigned)((count + per_block - 1) / per_block));
+  }
+}
+
 // alz_iir.hip: any section shape, channels [c_first, c_first + c_count)
 int launch_section(const SectionDev &sec, const BlockIO &io, hipStream_t stream,
                    const char **kernel_name);

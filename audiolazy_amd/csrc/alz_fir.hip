@@ -809,7 +809,7 @@ int launch_fir(const SectionDev &sec, const BlockIO &io, hipStream_t stream, boo
     const size_t lds = tap_bytes + (size_t)(cm_pad_host(kCmOut + hist) + 1 + cm_pad_host(kCmOut) + 1) * sizeof(double);
     if (lds > 60 * 1024) return ALZ_OK;
     const unsigned gyc = (unsigned)((io.n + kCmOut - 1) / kCmOut);
-    if (gyc > 65535u || io.c_count > 0x7fffffff) return ALZ_OK;
+    if (gyc > 65535u || io.c_count * 64 > kSliceItems) return ALZ_OK;   // (64 lanes per channel)
     hipLaunchKernelGGL(k_fir_cm, dim3((unsigned)io.c_count, gyc), dim3(64), lds, stream, p);
   } else if (sec.shared_sets && io.n < ((int64_t)1 << 31) - 4096 && io.n_inputs * 8 < ((int64_t)1 << 31) && io.channels * 8 < ((int64_t)1 << 31) &&
              io.sxn * 8 * kRingK < ((int64_t)1 << 31) &&
@@ -938,8 +938,9 @@ int launch_fir(const SectionDev &sec, const BlockIO &io, hipStream_t stream, boo
   hipLaunchKernelGGL(k_fir_state, dim3(gx, 8), dim3(64), 0, stream, p, xh_new);
   // only the channels of this launch were refreshed in xh_new: copy just those back
   if (io.c_first == 0 && io.c_count == io.channels) {
-    hipLaunchKernelGGL(k_copy_doubles, dim3((unsigned)((nx + 255) / 256)), dim3(256), 0, stream,
-                       sec.xh, xh_new, nx);
+    in_slices(nx, 256, [&](int64_t first, int64_t count, unsigned blocks) {
+      hipLaunchKernelGGL(k_copy_doubles, dim3(blocks), dim3(256), 0, stream, sec.xh + first, xh_new + first, count);
+    });
   } else {
     for (int k = 0; k < sec.nb - 1; ++k)
       hipLaunchKernelGGL(k_copy_doubles, dim3((unsigned)((io.c_count + 255) / 256)), dim3(256), 0,

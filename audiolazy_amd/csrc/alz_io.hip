@@ -25,13 +25,14 @@ struct MixArgs {
   int64_t n_sets, n_inputs, n;
   int64_t inner;       // extent of the fastest (contiguous) axis of out
   int64_t total;       // n * n_inputs
+  int64_t first;       // the launch's first output element
   int64_t y_outer, y_set, o_outer;   // strides in doubles
 };
 
 // One output element per lane.  Time-major: inner = input, outer = time, a set is n_inputs
 // further along the row.  Channel-major: inner = time, outer = input, a set is n_inputs rows down.
 __global__ __launch_bounds__(256) void k_mix(MixArgs p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = p.first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= p.total) return;
   const int64_t outer = i / p.inner, in = i - outer * p.inner;
   const double *src = p.y + outer * p.y_outer + in;
@@ -221,8 +222,10 @@ int alz_mix_dev(const double *y_dev, int64_t n_sets, int64_t n_inputs, int64_t n
   }
   alz::DeviceScope scope(device);
   if (!scope.ok) return alz::fail(ALZ_E_HIP, "hipSetDevice failed");
-  const unsigned grid = (unsigned)((p.total + 255) / 256);
-  hipLaunchKernelGGL(alz::k_mix, dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
+  alz::in_slices(p.total, 256, [&](int64_t first, int64_t, unsigned blocks) {
+    p.first = first;
+    hipLaunchKernelGGL(alz::k_mix, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
+  });
   ALZ_HIP_CHECK(hipGetLastError());
   return ALZ_OK;
 }
@@ -236,19 +239,21 @@ int alz_mix_tracks_dev(int n_tracks, const double *const *tracks_dev, const int6
   if (n_out == 0) return ALZ_OK;
   alz::DeviceScope scope(device);
   if (!scope.ok) return alz::fail(ALZ_E_HIP, "hipSetDevice failed");
-  const unsigned grid = (unsigned)((n_out + 255) / 256);
   int done = 0;
   do {   // at least one launch: with no track at all the output is `zero` everywhere
     alz::TrackArgs p;
     p.n_tracks = (n_tracks - done < alz::kMixTracks) ? n_tracks - done : alz::kMixTracks;
-    for (int k = 0; k < alz::kMixTracks; ++k) {
-      const bool on = k < p.n_tracks;
-      p.track[k] = on ? tracks_dev[done + k] : nullptr;
-      p.start[k] = on ? starts[done + k] : 0;
-      p.length[k] = on ? lengths[done + k] : 0;
-    }
-    p.first = done == 0; p.zero = zero; p.out = out_dev; p.n_out = n_out;
-    hipLaunchKernelGGL(alz::k_mix_tracks, dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
+    p.first = done == 0; p.zero = zero;
+    alz::in_slices(n_out, 256, [&](int64_t first, int64_t count, unsigned blocks) {
+      for (int k = 0; k < alz::kMixTracks; ++k) {
+        const bool on = k < p.n_tracks;
+        p.track[k] = on ? tracks_dev[done + k] : nullptr;
+        p.start[k] = on ? starts[done + k] - first : 0;      // (relative to the slice: negative where the track began before it)
+        p.length[k] = on ? lengths[done + k] : 0;
+      }
+      p.out = out_dev + first; p.n_out = count;
+      hipLaunchKernelGGL(alz::k_mix_tracks, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
+    });
     done += p.n_tracks;
   } while (done < n_tracks);
   ALZ_HIP_CHECK(hipGetLastError());
@@ -266,15 +271,12 @@ int alz_pcm_decode_dev(const void *raw_dev, int bits, int keep, int64_t n_sample
   if (n_samples == 0) return ALZ_OK;
   alz::DeviceScope scope(device);
   if (!scope.ok) return alz::fail(ALZ_E_HIP, "hipSetDevice failed");
-  const unsigned grid = (unsigned)(((n_samples + 3) / 4 + 255) / 256);
-  const unsigned char *raw = (const unsigned char *)raw_dev;
   hipStream_t st = (hipStream_t)stream;
-  switch (bits) {
-    case 8: hipLaunchKernelGGL(alz::k_pcm_decode<8>, dim3(grid), dim3(256), 0, st, raw, out_dev, n_samples, keep); break;
-    case 16: hipLaunchKernelGGL(alz::k_pcm_decode<16>, dim3(grid), dim3(256), 0, st, raw, out_dev, n_samples, keep); break;
-    case 24: hipLaunchKernelGGL(alz::k_pcm_decode<24>, dim3(grid), dim3(256), 0, st, raw, out_dev, n_samples, keep); break;
-    default: hipLaunchKernelGGL(alz::k_pcm_decode<32>, dim3(grid), dim3(256), 0, st, raw, out_dev, n_samples, keep); break;
-  }
+  void (*fn)(const unsigned char *, double *, int64_t, int) = bits == 8 ? alz::k_pcm_decode<8> : bits == 16 ? alz::k_pcm_decode<16>
+                                                              : bits == 24 ? alz::k_pcm_decode<24> : alz::k_pcm_decode<32>;
+  alz::in_slices(n_samples, 4 * 256, [&](int64_t first, int64_t count, unsigned blocks) {
+    hipLaunchKernelGGL(fn, dim3(blocks), dim3(256), 0, st, (const unsigned char *)raw_dev + first * (bits / 8), out_dev + first, count, keep);
+  });
   ALZ_HIP_CHECK(hipGetLastError());
   return ALZ_OK;
 }
@@ -297,6 +299,14 @@ int alz_pcm_encode_dev(const double *in_dev, int64_t n, int dfmt, int big_endian
     default: return alz::fail(ALZ_E_UNSUPPORTED, "dfmt must be one of b B h H i I l L f d");
   }
   if (n == 0) return ALZ_OK;
+  if (n > alz::kSliceItems) {      // (more than one launch can take)
+    for (int64_t first = 0; first < n; first += alz::kSliceItems) {
+      const int rc = alz_pcm_encode_dev(in_dev + first, n - first < alz::kSliceItems ? n - first : alz::kSliceItems, dfmt, big_endian,
+                                        (unsigned char *)out_dev + first * p.width, flags_dev, device, stream);
+      if (rc) return rc;
+    }
+    return ALZ_OK;
+  }
   alz::DeviceScope scope(device);
   if (!scope.ok) return alz::fail(ALZ_E_HIP, "hipSetDevice failed");
   hipStream_t st = (hipStream_t)stream;

@@ -664,6 +664,13 @@ static int launch_lpc(const double *sig, int64_t n_frames, int frame_len, int64_
   return ALZ_OK;
 }
 
+// frames of one launch with `per_frame` (or 64) work-items per frame: a multiple of 64, which keeps the alignment that the staged
+// kernel asks for, where there are as many
+static int64_t frame_slice(int64_t per_frame) {
+  const int64_t slice = kSliceItems / (per_frame > 64 ? per_frame : 64);
+  return slice >= 64 ? slice / 64 * 64 : slice > 1 ? slice : 1;
+}
+
 }  // namespace alz
 
 extern "C" {
@@ -673,6 +680,15 @@ int alz_lpc_kautocor_dev_ex(const double *sig_dev, int64_t n_frames, int frame_l
                             void *stream) {
   if (!sig_dev || !coefs_dev || !err_dev || !status_dev) return alz::fail(ALZ_E_ARG, "NULL argument");
   if (n_frames < 0 || frame_len < 1 || hop < 0 || order < 0) return alz::fail(ALZ_E_ARG, "lpc: bad frame geometry");
+  // (larger batches than one launch takes)
+  if (const int64_t slice = alz::frame_slice((int64_t)order + 1); n_frames > slice) {
+    for (int64_t f = 0; f < n_frames; f += slice) {
+      const int rc = alz_lpc_kautocor_dev_ex(sig_dev + f * hop, n_frames - f < slice ? n_frames - f : slice, frame_len, hop, order,
+                                             coefs_dev + f * (order + 1), err_dev + f, status_dev + f, flags, device, stream);
+      if (rc) return rc;
+    }
+    return ALZ_OK;
+  }
   int prev = 0;
   ALZ_HIP_CHECK(hipGetDevice(&prev));
   if (prev != device) ALZ_HIP_CHECK(hipSetDevice(device));
@@ -759,6 +775,15 @@ int alz_levinson_dev_ex(const double *r_dev, int64_t n_frames, int n_lags, int o
   if (!r_dev || !coefs_dev || !err_dev || !status_dev) return alz::fail(ALZ_E_ARG, "NULL argument");
   if (n_lags < 1) return alz::fail(ALZ_E_ARG, "levinson: need at least lag 0");
   if (n_frames < 0 || order < 0) return alz::fail(ALZ_E_ARG, "levinson: bad geometry");
+  // (larger batches than one launch takes)
+  if (const int64_t slice = alz::frame_slice((int64_t)order + 1); n_frames > slice) {
+    for (int64_t f = 0; f < n_frames; f += slice) {
+      const int rc = alz_levinson_dev_ex(r_dev + f * n_lags, n_frames - f < slice ? n_frames - f : slice, n_lags, order,
+                                         coefs_dev + f * (order + 1), err_dev + f, status_dev + f, flags, device, stream);
+      if (rc) return rc;
+    }
+    return ALZ_OK;
+  }
   int prev = 0;
   ALZ_HIP_CHECK(hipGetDevice(&prev));
   if (prev != device) ALZ_HIP_CHECK(hipSetDevice(device));
@@ -791,6 +816,15 @@ int alz_acorr_dev(const double *sig_dev, int64_t n_frames, int frame_len, int64_
                   double *r_dev, int device, void *stream) {
   if (!sig_dev || !r_dev) return alz::fail(ALZ_E_ARG, "NULL argument");
   if (n_frames < 0 || frame_len < 1 || hop < 0 || max_lag < 0) return alz::fail(ALZ_E_ARG, "acorr: bad frame geometry");
+  // (larger batches than one launch takes)
+  if (const int64_t slice = alz::frame_slice((int64_t)max_lag + 1); n_frames > slice) {
+    for (int64_t f = 0; f < n_frames; f += slice) {
+      const int rc = alz_acorr_dev(sig_dev + f * hop, n_frames - f < slice ? n_frames - f : slice, frame_len, hop, max_lag,
+                                   r_dev + f * (max_lag + 1), device, stream);
+      if (rc) return rc;
+    }
+    return ALZ_OK;
+  }
   int prev = 0;
   ALZ_HIP_CHECK(hipGetDevice(&prev));
   if (prev != device) ALZ_HIP_CHECK(hipSetDevice(device));
@@ -810,7 +844,16 @@ int alz_lag_matrix_dev(const double *sig_dev, int64_t n_frames, int frame_len, i
   if (max_lag < 0 || frame_len < 1 || hop < 0 || n_frames < 0) return alz::fail(ALZ_E_ARG, "bad lag_matrix shape");
   if (max_lag >= frame_len) return alz::fail(ALZ_E_ARG, "Block length should be higher than order");
   const int64_t cells = (int64_t)(max_lag + 1) * (max_lag + 1);
-  if (n_frames > 0 && cells > (INT64_C(0x7fffffff) * 256) / n_frames) return alz::fail(ALZ_E_ARG, "lag_matrix batch too large");
+  if (cells > alz::kSliceItems) return alz::fail(ALZ_E_UNSUPPORTED, "lag_matrix: max_lag too large");
+  // (larger batches than one launch takes)
+  if (const int64_t slice = alz::frame_slice(cells); n_frames > slice) {
+    for (int64_t f = 0; f < n_frames; f += slice) {
+      const int rc = alz_lag_matrix_dev(sig_dev + f * hop, n_frames - f < slice ? n_frames - f : slice, frame_len, hop, max_lag,
+                                        phi_dev + f * cells, device, stream);
+      if (rc) return rc;
+    }
+    return ALZ_OK;
+  }
   int prev = 0;
   ALZ_HIP_CHECK(hipGetDevice(&prev));
   if (prev != device) ALZ_HIP_CHECK(hipSetDevice(device));
