@@ -143,6 +143,19 @@ struct DeviceGuard {
   }
 };
 
+// the most channels a bank can have: one double each of these fills far more than a device
+constexpr int64_t kMaxChannels = INT64_C(1) << 40;
+
+// the end of an entry point that allocates host memory by the size of the bank: no exception leaves the library
+int out_of_memory() {
+  try {
+    return fail(ALZ_E_NOMEM, "out of host memory");
+  } catch (...) {
+    return ALZ_E_NOMEM;
+  }
+}
+#define ALZ_END_OF_ENTRY catch (...) { return out_of_memory(); }
+
 // host [rows = channels][cols] (row-major)  <->  device [cols][channels]
 void transpose_to_dev_order(const double *src, std::vector<double> &dst, int64_t rows, int64_t cols) {
   dst.resize((size_t)(rows * cols));
@@ -217,7 +230,7 @@ int alz_device_sync(int device) {
 
 int alz_bank_create(int64_t n_sets, int64_t n_inputs, int mode, int n_sections, const int *nb,
                     const int *na, const double *b_host, const double *a_host, int device,
-                    alz_bank_t **out) {
+                    alz_bank_t **out) try {
   if (!out) return fail(ALZ_E_ARG, "out is NULL");
   *out = nullptr;
   if (n_sets < 1 || n_inputs < 1 || n_sections < 1 || !nb || !na || !b_host || !a_host)
@@ -225,6 +238,8 @@ int alz_bank_create(int64_t n_sets, int64_t n_inputs, int mode, int n_sections, 
   if (mode != ALZ_BANK_DIAGONAL && mode != ALZ_BANK_OUTER) return fail(ALZ_E_ARG, "bad bank mode");
   if (mode == ALZ_BANK_DIAGONAL && n_sets != n_inputs && n_sets != 1)
     return fail(ALZ_E_ARG, "DIAGONAL bank needs n_sets == n_inputs (or 1 shared set)");
+  if (n_inputs > kMaxChannels || n_sets > kMaxChannels || (mode == ALZ_BANK_OUTER && n_inputs > kMaxChannels / n_sets))
+    return fail(ALZ_E_ARG, "too many channels");
   int64_t tb = 0, ta = 0;
   for (int s = 0; s < n_sections; ++s) {
     if (nb[s] < 1 || na[s] < 1) return fail(ALZ_E_ARG, "every section needs nb >= 1 and na >= 1");
@@ -243,6 +258,12 @@ int alz_bank_create(int64_t n_sets, int64_t n_inputs, int mode, int n_sections, 
 
   alz_bank *h = new (std::nothrow) alz_bank();
   if (!h) return fail(ALZ_E_NOMEM, "out of host memory");
+  struct Unfinished {                     // (an exception on the way takes the handle and what it holds with it)
+    alz_bank *h;
+    ~Unfinished() {
+      if (h) alz_bank_destroy(h);
+    }
+  } unfinished{h};
   h->device = device;
   h->n_sets = n_sets;
   h->n_inputs = n_inputs;
@@ -257,10 +278,10 @@ int alz_bank_create(int64_t n_sets, int64_t n_inputs, int mode, int n_sections, 
     h->thx += nb[s] - 1;
     h->thy += na[s] - 1;
   }
+  if (h->channels > kMaxChannels / (1 + (h->thx > h->thy ? h->thx : h->thy))) return fail(ALZ_E_NOMEM, "the bank's state is larger than any device");
 
   DeviceGuard g(device);
   if (!g.ok) {
-    delete h;
     return fail(ALZ_E_HIP, "hipSetDevice failed");
   }
   // coefficients, tap-major on the device: section s, tap k, set q at
@@ -275,13 +296,11 @@ int alz_bank_create(int64_t n_sets, int64_t n_inputs, int mode, int n_sections, 
       hipMalloc((void **)&h->a_dev, at.size() * 8) != hipSuccess ||
       hipMalloc((void **)&h->xh_dev, xs) != hipSuccess ||
       hipMalloc((void **)&h->yh_dev, ys) != hipSuccess) {
-    alz_bank_destroy(h);
     return fail(ALZ_E_NOMEM, "hipMalloc failed while creating the bank");
   }
   if (hipMemcpy(h->b_dev, bt.data(), bt.size() * 8, hipMemcpyHostToDevice) != hipSuccess ||
       hipMemcpy(h->a_dev, at.data(), at.size() * 8, hipMemcpyHostToDevice) != hipSuccess ||
       hipMemset(h->xh_dev, 0, xs) != hipSuccess || hipMemset(h->yh_dev, 0, ys) != hipSuccess) {
-    alz_bank_destroy(h);
     return fail(ALZ_E_HIP, "coefficient upload failed");
   }
 
@@ -358,9 +377,11 @@ int alz_bank_create(int64_t n_sets, int64_t n_inputs, int mode, int n_sections, 
     }
     (void)hipGetLastError();
   }
+  unfinished.h = nullptr;
   *out = h;
   return ALZ_OK;
 }
+ALZ_END_OF_ENTRY
 
 int alz_bank_destroy(alz_bank_t *h) {
   if (!h) return ALZ_OK;
@@ -444,7 +465,7 @@ static int put_state(alz_bank *h, const double *xh_host, const double *yh_host) 
   return ALZ_OK;
 }
 
-int alz_bank_reset(alz_bank_t *h, double zero) {
+int alz_bank_reset(alz_bank_t *h, double zero) try {
   if (!h) return fail(ALZ_E_ARG, "NULL handle");
   DeviceGuard g(h->device);
   ALZ_HIP_CHECK(hipDeviceSynchronize());
@@ -453,13 +474,15 @@ int alz_bank_reset(alz_bank_t *h, double zero) {
   std::vector<double> yh((size_t)(h->channels * (h->thy > 0 ? h->thy : 1)), zero);
   return put_state(h, xh.data(), yh.data());
 }
+ALZ_END_OF_ENTRY
 
-int alz_bank_set_state(alz_bank_t *h, const double *xh_host, const double *yh_host) {
+int alz_bank_set_state(alz_bank_t *h, const double *xh_host, const double *yh_host) try {
   if (!h) return fail(ALZ_E_ARG, "NULL handle");
   DeviceGuard g(h->device);
   ALZ_HIP_CHECK(hipDeviceSynchronize());
   return put_state(h, xh_host, yh_host);
 }
+ALZ_END_OF_ENTRY
 
 // The one-pass time-parallel kernel (alz_look.hip) reports a wait that ran out in a word of pinned host memory per
 // section.  Every entry point that hands results to the caller looks at it -- after its synchronisation where it has
@@ -496,7 +519,7 @@ static int take_look_error(alz_bank_t *h) {
                : ALZ_OK;
 }
 
-int alz_bank_get_state(alz_bank_t *h, double *xh_host, double *yh_host) {
+int alz_bank_get_state(alz_bank_t *h, double *xh_host, double *yh_host) try {
   if (!h) return fail(ALZ_E_ARG, "NULL handle");
   DeviceGuard g(h->device);
   ALZ_HIP_CHECK(hipDeviceSynchronize());
@@ -520,12 +543,13 @@ int alz_bank_get_state(alz_bank_t *h, double *xh_host, double *yh_host) {
   }
   return ALZ_OK;
 }
+ALZ_END_OF_ENTRY
 
 static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, int64_t n, int layout,
                             int64_t ldx, int64_t ldy, void *stream, bool capturing);
 
 int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev, int64_t n, int layout,
-                         int64_t ldx, int64_t ldy, void *stream) {
+                         int64_t ldx, int64_t ldy, void *stream) try {
   // The one-pass time-parallel kernel (alz_look.hip) is the one kernel of the library whose workgroups wait for each
   // other; its waits are bounded, and a launch that gave up (its workgroups were not all resident in time: foreign work
   // on the device) has written a bad block and a bad state.  ALZ_LOOK_CHECK_CALL (default): this call notices -- it keeps
@@ -576,6 +600,7 @@ int alz_bank_process_dev(alz_bank_t *h, const double *x_dev, double *y_dev, int6
   if (rc == ALZ_OK && h && n >= 2) h->state_consistent = true;
   return rc;
 }
+ALZ_END_OF_ENTRY
 
 static int process_dev_impl(alz_bank_t *h, const double *x_dev, double *y_dev, int64_t n, int layout,
                             int64_t ldx, int64_t ldy, void *stream, bool capturing) {
@@ -1108,7 +1133,7 @@ static int host_pipeline(alz_bank_t *h, const double *x_host, double *y_host, in
 }
 
 int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, int64_t n, int layout,
-                          int64_t ldx, int64_t ldy) {
+                          int64_t ldx, int64_t ldy) try {
   if (!h || !x_host || !y_host) return fail(ALZ_E_ARG, "NULL argument");
   if (n <= 0) return n == 0 ? ALZ_OK : fail(ALZ_E_ARG, "negative block length");
   if (layout != ALZ_TIME_MAJOR && layout != ALZ_CHAN_MAJOR) return fail(ALZ_E_ARG, "bad layout");
@@ -1148,6 +1173,7 @@ int alz_bank_process_host(alz_bank_t *h, const double *x_host, double *y_host, i
   if (const int lrc = take_look_error(h)) return lrc;
   return rows_to_host(h, y_host, ldy, h->stage_y, lsy, out_cols, out_rows);
 }
+ALZ_END_OF_ENTRY
 
 int alz_bank_set_fused(alz_bank_t *h, int on) {
   if (!h) return fail(ALZ_E_ARG, "NULL handle");

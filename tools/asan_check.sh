@@ -12,7 +12,7 @@ export ASAN_OPTIONS=detect_leaks=0:protect_shadow_gap=0:halt_on_error=1:abort_on
 export ALZ_LIBRARY=$R/tools/variants/libalzhip_asan.so LD_PRELOAD=$RT
 cd $R
 case ${1:-cpu} in
-  cpu) python -m pytest tests/test_cabi_cpu.py tests/test_bench_cpu.py -x -q -m "not gpu" 2>&1 | tail -5 ;;
+  cpu) python -m pytest tests/test_cabi_cpu.py tests/test_bench_cpu.py tests/test_bank_sizes_cpu.py tests/test_lpc_geometry_cpu.py tests/test_timevar_pitch_cpu.py -x -q -m "not gpu" 2>&1 | tail -5 ;;
   gpu) unset LD_PRELOAD; export ALZ_LIBRARY=$R/tools/variants/libalzhip_ubsan.so
        python -c "import __graft_entry__ as g; g.smoke(); print('smoke ok under host UBSan')" 2>&1 | tail -3
        python -m pytest tests/test_gpu_scan.py tests/test_gpu_mid.py tests/test_gpu_bank.py tests/test_gpu_host_path.py -x -q -m gpu 2>&1 | tail -5
