@@ -455,6 +455,8 @@ class FilterBank(object):
           or (out.shape != shape and not (flat and self.channels == 1 and out.shape == (n,)))):
         raise ValueError("out must be a writable C-contiguous float64 array of shape %s" % (shape,))
       y = out
+      if np.may_share_memory(x, y) and (x.ctypes.data, x.nbytes) != (y.ctypes.data, y.nbytes):
+        x = x.copy()        # (results of one chunk are written while the next one is still read)
     if n == 0:
       return y
     ldx = self.n_inputs if lay == _ffi.TIME_MAJOR else n

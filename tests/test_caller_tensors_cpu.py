@@ -211,3 +211,26 @@ def test_empty_blocks(lib):
   coefs, err, status = kautocor_frames(dev(479), 480, 8)
   assert (tuple(coefs.shape), tuple(err.shape), tuple(status.shape)) == ((0, 9), (0,), (0,))
   assert not lib.calls
+
+
+@pytest.mark.parametrize("shift", [-3, -1, 0, 1, 3])
+def test_process_on_arrays_that_overlap(lib, shift):
+  """The result may be the input itself; a result that lies across it must not be written while the input is still read."""
+  bank = FilterBank([([1.], [1., .5])], n_inputs=4)
+  base = np.arange(80.).reshape(20, 4)
+  x, out = base[5:15], base[5 + shift:15 + shift]
+  del lib.calls[:]
+  bank.process(x, out=out)
+  (name, args), = lib.calls
+  read = np.ctypeslib.as_array(args[1], (10, 4))
+  assert np.array_equal(read, x) and ctypes.cast(args[2], ctypes.c_void_p).value == out.ctypes.data
+  assert np.shares_memory(read, out) == (shift == 0)
+
+
+def test_process_on_a_larger_result_that_begins_with_the_input(lib):
+  bank = FilterBank([([1.], np.array([[1., .5], [1., .25], [1., .125]]))], n_inputs=1, mode="outer")
+  base = np.arange(30.)
+  del lib.calls[:]
+  bank.process(base[:10].reshape(10, 1), out=base.reshape(10, 3))
+  (name, args), = lib.calls
+  assert not np.shares_memory(np.ctypeslib.as_array(args[1], (10, 1)), base)
