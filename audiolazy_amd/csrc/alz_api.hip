@@ -62,6 +62,7 @@ int grow_buffer(Kept *kept, bool capturing, double **ptr, uint64_t *have, uint64
   *have = 0;
   if (hipMalloc((void **)ptr, need) != hipSuccess) {
     *ptr = nullptr;
+    (void)hipGetLastError();              // (else the next launch's check reports it)
     return fail(ALZ_E_NOMEM, "hipMalloc failed for " + std::to_string(need) + " bytes");
   }
   *have = need;
